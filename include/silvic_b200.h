@@ -90,7 +90,8 @@ typedef struct sb2_dataset {
 
 /* ObjectiveSetup (crates/silvic-core/src/backend/mod.rs:58-71). Lambdarank (objective/lambdarank.rs) takes the
  * dataset's query boundaries; its per-query inverse max DCGs are computed at load from the labels. */
-enum { SB2_REGRESSION = 0, SB2_BINARY = 1, SB2_LAMBDARANK = 2 };
+enum { SB2_REGRESSION = 0, SB2_BINARY = 1, SB2_LAMBDARANK = 2,
+       SB2_DISTILL = 3 }; /* no counterpart in the reference: distillation over the dataset's queries (sb2_set_teacher) */
 typedef struct sb2_objective {
     int32_t kind;
     int32_t pad_;
@@ -188,7 +189,7 @@ typedef struct sb2_split_info {
 /* Training parameters (crates/silvic-core/src/config.rs:73-116, defaults :123-165), the subset this backend
  * trains with. sb2_default_params() fills the reference defaults. */
 typedef struct sb2_params {
-    int32_t objective;            /* SB2_REGRESSION / SB2_BINARY / SB2_LAMBDARANK */
+    int32_t objective;            /* SB2_REGRESSION / SB2_BINARY / SB2_LAMBDARANK / SB2_DISTILL */
     int32_t num_iterations;
     double learning_rate;
     int32_t num_leaves;
@@ -405,6 +406,76 @@ int sb2_bin_dense(sb2_backend* b, const void* values, int value_bytes, uint64_t 
  * dominant bin causes no bank conflict, and on B200 the per-element test costs more issue slots than the skipped
  * atomics save. 0: every tile skips. Takes effect at the next sb2_load. */
 int sb2_set_dominant_share(sb2_backend* b, double share);
+
+/* ---- softmax over lists of candidates ----------------------------------------------------------------------- */
+
+/* No counterpart in the reference: a language model's logits, or a ranker's scores, as lists of candidates, and the
+ * operators that make a teacher of the first and a student of the second. A list is a row of a dense matrix (one
+ * position's logits over a vocabulary) or a run of a flat array between two boundaries (a query's documents).
+ *
+ * Every pointer named _dev is memory of the handle's device (else SB2_EDATA). The calls enqueue one kernel on `stream`
+ * (a cudaStream_t of that device; NULL: its default stream), allocate nothing, wait for nothing, and may be captured
+ * into a CUDA graph; the caller orders them after the writes of their inputs. Calls on different streams do not
+ * disturb one another. The current device stays as it was.
+ *
+ * Values: -inf is a masked entry (probability 0); a list that holds a NaN or +inf has NaN results; -0 equals 0. A list
+ * of no entries, or of masked ones only, is empty: log sum -inf, entropy 0, no alternatives, loss and gradients 0.
+ * Sums and softmax statistics are f32. */
+enum { SB2_F32 = 0, SB2_BF16 = 1, SB2_F16 = 2 };
+typedef struct sb2_lists {
+    const void* scores_dev;
+    int32_t type;                   /* of the scores: SB2_F32 / SB2_BF16 / SB2_F16 */
+    uint32_t num_lists;
+    uint64_t width;                 /* dense: entries of a list (below 2^31); with boundaries: entries behind scores_dev */
+    uint64_t stride;                /* dense: entries from one list to the next (at least width for 2 lists and more) */
+    const uint32_t* boundaries_dev; /* NULL: dense; else num_lists + 1 boundaries that do not decrease (what lies
+                                       outside the entries is cut off), as sb2_dataset's query_boundaries */
+} sb2_lists;
+
+/* A teacher's top entries of each list: row i of `ids_dev` and `logits_dev` starts at i * stride. An id outside the
+ * list (-1 by custom) is padding; an id given twice counts with both its logits. */
+typedef struct sb2_teacher {
+    const int32_t* ids_dev;
+    const void* logits_dev;
+    int32_t type;                   /* of the logits */
+    uint32_t top;                   /* 1 .. 128 */
+    uint64_t stride;                /* at least top */
+    const float* log_sum_dev;       /* NULL: the top is the whole teacher (renormalised); else num_lists log sums,
+                                       ln sum exp(t / temperature) over the teacher's whole list (0 for logits that are
+                                       log probabilities), and the rest of its mass is one more class */
+} sb2_teacher;
+
+/* softmax(z / temperature) of every list z: log_sum_dev [num_lists] ln sum exp(z / temperature); entropy_dev
+ * [num_lists] in nats; given_out_dev [num_lists, num_given] the log probabilities of the entries given_dev
+ * [num_lists, num_given] (-inf for an index outside the list); top_ids_dev and top_out_dev [num_lists, top] the most
+ * likely entries, likeliest first, ties by the lower index, and their log probabilities (-1 and -inf behind the last
+ * entry that is not masked; in a list with a NaN the alternatives' indices say nothing). log_sum_dev and entropy_dev
+ * may be NULL. top is at most 128 (else SB2_EUNSUPPORTED). */
+int sb2_log_probs(sb2_backend* b, const sb2_lists* lists, double temperature, const int32_t* given_dev,
+                  uint32_t num_given, uint32_t top, float* given_out_dev, float* entropy_dev, float* log_sum_dev,
+                  int32_t* top_ids_dev, float* top_out_dev, void* stream);
+
+/* The distillation loss of every list and its derivatives. With the student's p = softmax(z / T), the teacher's q
+ * over its top, r = 1 - sum q the teacher's rest (0 without log_sum_dev, or where the student has no mass outside the
+ * top), P the student's mass outside the top and Q = sum q + r:
+ *   loss_dev [num_lists]  weight * (sum q (ln q - ln p) + r (ln r - ln P))
+ *   grad_dev              d loss / d z_j = weight / T * (Q p_j - q_j) in the top, weight / T * p_j (Q - r / P) elsewhere
+ *   hess_dev              weight / T^2 * Q p_j (1 - p_j), the diagonal of the softmax's own second derivative
+ * weight_dev [num_lists] may be NULL (1 each), so may any of the three outputs. Gradient and hessian have the scores'
+ * type; with boundaries their layout too, dense rows start grad_stride entries apart (0: as the scores'), and entries
+ * between the lists stay as they are. They must not overlap the scores or each other (SB2_EDATA). A list whose
+ * teacher has no entry in it has loss and gradients 0; a teacher's entry that the student masks has loss +inf. */
+int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* teacher, double temperature,
+                const float* weight_dev, float* loss_dev, void* grad_dev, void* hess_dev, uint64_t grad_stride,
+                void* stream);
+
+/* The teacher of the SB2_DISTILL objective, after sb2_load with it (which takes the dataset's query boundaries) and
+ * before gradients or training: num_queries rows of `top` ids (a row's index within its query, -1: padding) and
+ * logits in host memory, log_sum NULL or num_queries values, as in sb2_teacher. A training iteration's gradients and
+ * hessians are then sb2_distill's with weight 1, times each row's weight in a weighted dataset. Queries may have any
+ * length. An id outside its query, a logit that is NaN or +inf or a log sum that is not finite returns SB2_EDATA. */
+int sb2_set_teacher(sb2_backend* b, const int32_t* ids, const float* logits, const float* log_sum, uint64_t num_lists,
+                    uint32_t top, double temperature);
 
 /* ---- multi-GPU --------------------------------------------------------------------------------------------- */
 

@@ -9,14 +9,18 @@ silvic's boosting loop with every split on the device. The compiled library live
 from ._abi import SilvicError, load_library
 from .backend import B200Backend, Model, Tree, init_score, params_from_dict, train
 from .dataset import BinnedDataset, FeatureGroup, FeatureMeta, numerical_mapper
+from .lists import Distilled, LogProbs, TeacherTop
 
 __all__ = [
     "B200Backend",
     "BinnedDataset",
+    "Distilled",
     "FeatureGroup",
     "FeatureMeta",
+    "LogProbs",
     "Model",
     "SilvicError",
+    "TeacherTop",
     "Tree",
     "init_score",
     "load_library",

@@ -13,7 +13,8 @@ LIBRARY = Path(__file__).resolve().parent / "_lib" / "libsilvic_b200.so"
 
 OK, ECONFIG, EDATA, EINTERNAL, EDEVICE, ECOLLECTIVE, EMODEL, EUNSUPPORTED = range(8)
 NUMERICAL, CATEGORICAL, TRIVIAL = 0, 1, 2
-REGRESSION, BINARY, LAMBDARANK = 0, 1, 2
+REGRESSION, BINARY, LAMBDARANK, DISTILL = 0, 1, 2, 3
+F32, BF16, F16 = 0, 1, 2
 EXCHANGE_AUTO, EXCHANGE_NCCL = 0, 1
 LEFT, RIGHT = 0, 1
 
@@ -217,6 +218,16 @@ class TreeView(C.Structure):
     ]
 
 
+class Lists(C.Structure):
+    _fields_ = [("scores_dev", C.c_void_p), ("type", C.c_int32), ("num_lists", C.c_uint32), ("width", C.c_uint64),
+                ("stride", C.c_uint64), ("boundaries_dev", C.c_void_p)]
+
+
+class Teacher(C.Structure):
+    _fields_ = [("ids_dev", C.c_void_p), ("logits_dev", C.c_void_p), ("type", C.c_int32), ("top", C.c_uint32),
+                ("stride", C.c_uint64), ("log_sum_dev", C.c_void_p)]
+
+
 # Exported functions: name -> (restype, argtypes). Every symbol the header declares.
 P = C.POINTER
 VP = C.c_void_p
@@ -268,6 +279,9 @@ SIGNATURES = {
     "sb2_model_tree_seconds": (C.c_int, [VP, P(C.c_double), C.c_size_t]),
     "sb2_bin_dense": (C.c_int, [VP, VP, C.c_int, C.c_uint64, C.c_uint32, C.c_int, P(Feature), C.c_uint32, P(Group),
                                 C.c_uint32, P(P(C.c_uint8))]),
+    "sb2_log_probs": (C.c_int, [VP, P(Lists), C.c_double, VP, C.c_uint32, C.c_uint32, VP, VP, VP, VP, VP, VP]),
+    "sb2_distill": (C.c_int, [VP, P(Lists), P(Teacher), C.c_double, VP, VP, VP, VP, C.c_uint64, VP]),
+    "sb2_set_teacher": (C.c_int, [VP, P(C.c_int32), P(C.c_float), P(C.c_float), C.c_uint64, C.c_uint32, C.c_double]),
 }
 
 _lib = None

@@ -15,6 +15,7 @@ import numpy as np
 
 from . import _abi
 from .dataset import BinnedDataset
+from .lists import Distilled, LogProbs, TeacherTop
 
 _PARAM_ALIASES = {
     "objective": ["objective_type", "app", "application", "loss"],
@@ -51,7 +52,7 @@ _PARAM_ALIASES = {
 }
 _OBJECTIVES = {"regression": _abi.REGRESSION, "regression_l2": _abi.REGRESSION, "l2": _abi.REGRESSION,
                "mean_squared_error": _abi.REGRESSION, "mse": _abi.REGRESSION, "binary": _abi.BINARY,
-               "lambdarank": _abi.LAMBDARANK}
+               "lambdarank": _abi.LAMBDARANK, "distill": _abi.DISTILL}
 # Accepted for LightGBM compatibility, no effect (crates/silvic-core/src/config.rs NO_EFFECT_KEYS), plus the ones
 # that select this backend or describe binning, which happens before training.
 _IGNORED = {"force_row_wise", "force_col_wise", "deterministic", "histogram_pool_size", "feature_pre_filter",
@@ -131,6 +132,7 @@ class B200Backend:
         if code != _abi.OK:
             raise _abi.SilvicError(code, _abi.global_error())
         self._h = h
+        self._device = device
         self._data: BinnedDataset | None = None
 
     def close(self):
@@ -256,6 +258,77 @@ class B200Backend:
         out = np.empty(self._data.num_rows, dtype=np.float32)
         self._check(self._lib.sb2_scores(self._h, dataset, out.ctypes.data_as(C.POINTER(C.c_float)), len(out)))
         return out
+
+    # ---- softmax over lists of candidates (no counterpart in the reference) ----
+    def log_probs(self, scores, *, given=None, top: int = 0, temperature: float = 1.0, boundaries=None) -> LogProbs:
+        """softmax(scores / temperature) of every list (`sb2_log_probs`): the log probabilities of the `given`
+        entries (int32 [lists, n] or [lists]), the entropy, the log sum and the `top` likeliest entries (at most 128).
+        `scores`: a CUDA tensor, f32, bf16 or f16, of a list a row, or 1-D with `boundaries` (int32 or uint32, lists
+        + 1). Runs on torch's current stream of the handle's device, without waiting; may be captured into a graph."""
+        import torch
+
+        from . import lists as L
+
+        arg = L.lists_arg(scores, boundaries)
+        n = arg.num_lists
+        given = None if given is None else L.given_arg(given, n)
+        num_given = 0 if given is None else given.shape[1]
+        if not 0 <= top <= L.MAX_TOP:
+            raise ValueError(f"{top} alternatives; 0 to {L.MAX_TOP} are given")
+        L.check_device(self._device, [t for t in (scores, boundaries, given) if t is not None])
+        f32 = dict(dtype=torch.float32, device=scores.device)
+        out = LogProbs(torch.empty((n, num_given), **f32) if given is not None else None, torch.empty(n, **f32),
+                       torch.empty(n, **f32),
+                       torch.empty((n, top), dtype=torch.int32, device=scores.device) if top else None,
+                       torch.empty((n, top), **f32) if top else None)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._check(self._lib.sb2_log_probs(self._h, C.byref(arg), temperature, ptr(given), num_given, top,
+                                            ptr(out.given), ptr(out.entropy), ptr(out.log_sum), ptr(out.top_ids),
+                                            ptr(out.top), torch.cuda.current_stream(scores.device).cuda_stream))
+        return out
+
+    def distill(self, scores, teacher: TeacherTop, *, boundaries=None, weight=None, gradient: bool = True,
+                hessian: bool = False) -> Distilled:
+        """The distillation loss of every list against a teacher's top logits, its gradient and the softmax's own
+        hessian diagonal with respect to `scores` (`sb2_distill`, which has the formulas). `scores` and `boundaries`
+        as in `log_probs`; `weight` (f32 [lists]) multiplies a list's loss and derivatives (a loss's upstream
+        gradient, say). Gradient and hessian have the scores' type and shape, in memory of their own. Runs on torch's
+        current stream of the handle's device, without waiting; may be captured into a graph."""
+        import torch
+
+        from . import lists as L
+
+        arg = L.lists_arg(scores, boundaries)
+        n = arg.num_lists
+        t, keep = L.teacher_arg(teacher, n)
+        if weight is not None:
+            weight = L.per_list_arg(weight, n, "weight")
+        L.check_device(self._device, keep + [x for x in (scores, boundaries, weight) if x is not None])
+        # Gradients of padded rows are padded alike, so that both sides' rows start on the same boundaries; rows cut
+        # from far wider ones (a stride of more than the width and 64) lie one behind the other.
+        stride = 0 if boundaries is not None else arg.stride if arg.stride <= arg.width + 64 else arg.width
+
+        def empty():
+            if boundaries is not None or n == 0:
+                return torch.empty_like(scores, memory_format=torch.contiguous_format)
+            return torch.empty((n, stride), dtype=scores.dtype, device=scores.device)[:, : arg.width]
+
+        out = Distilled(torch.empty(n, dtype=torch.float32, device=scores.device), empty() if gradient else None,
+                        empty() if hessian else None)
+        ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+        self._check(self._lib.sb2_distill(self._h, C.byref(arg), C.byref(t), teacher.temperature, ptr(weight),
+                                          ptr(out.loss), ptr(out.gradient), ptr(out.hessian), stride,
+                                          torch.cuda.current_stream(scores.device).cuda_stream))
+        return out
+
+    def set_teacher(self, teacher: TeacherTop):
+        """sb2_set_teacher: the teacher of the loaded `distill` objective, a row of numpy arrays a query."""
+        from .lists import host_teacher
+
+        ids, logits, log_sum = host_teacher(teacher)
+        f32 = lambda a: None if a is None else a.ctypes.data_as(C.POINTER(C.c_float))  # noqa: E731
+        self._check(self._lib.sb2_set_teacher(self._h, ids.ctypes.data_as(C.POINTER(C.c_int32)), f32(logits),
+                                              f32(log_sum), ids.shape[0], ids.shape[1], teacher.temperature))
 
     # ---- state access for tests (the reference's CpuBackend tests read the same fields) ----
     def read_partition(self, n: int | None = None) -> np.ndarray:
@@ -480,12 +553,15 @@ def init_score(params: _abi.Params, label: np.ndarray, weight: np.ndarray | None
     return out.value
 
 
-def train(params: dict, train_set: BinnedDataset, device: int = 0) -> Model:
-    """`silvic.train(params, Dataset)` on one B200: every boosting iteration on the device."""
+def train(params: dict, train_set: BinnedDataset, device: int = 0, teacher: TeacherTop | None = None) -> Model:
+    """`silvic.train(params, Dataset)` on one B200: every boosting iteration on the device. The `distill` objective
+    (no counterpart in the reference) learns `teacher`'s top logits over the dataset's queries."""
     p = params_from_dict(params)
     backend = B200Backend(device)
     try:
         backend.load(train_set, p.objective, p.sigmoid, p)
+        if teacher is not None:
+            backend.set_teacher(teacher)
         return backend.train(p, init_score(p, train_set.label, train_set.weight))
     finally:
         backend.close()

@@ -101,6 +101,11 @@ struct sb2_backend {
     // lambdarank: the queries and the host-computed tables the gradient kernel reads (RankArgs)
     DeviceBuffer rk_bounds, rk_queries, rk_imdcg, rk_gain, rk_discount, rk_table;
     RankArgs ranking{};
+    // distillation: the queries (rk_bounds) and the teacher of sb2_set_teacher
+    DeviceBuffer teach_ids, teach_logits, teach_log_sum;
+    TeacherArgs teacher{};                    // top 0: none set
+    float teacher_inv_t = 1.0f;
+    std::vector<uint32_t> queries;            // the boundaries on the host, to check a teacher's ids against
     std::vector<double> rank_gain;            // the loaded label gains, to check training parameters against
     DeviceBuffer api_spec;                    // the QuantSpec of the last sb2_quantize
     sb2_quant_spec api_spec_host{};
@@ -188,6 +193,20 @@ struct sb2_backend {
         r.hess = hess.as<float>();
         r.packed = packed.as<int32_t>();
         r.rank = ranking;
+        if (objective.kind == SB2_DISTILL) {
+            DistillArgs& d = r.distill;
+            d.l.scores = r.scores;
+            d.l.type = SB2_F32;
+            d.l.lists = static_cast<uint32_t>(queries.size() - 1);
+            d.l.width = num_rows;
+            d.l.bounds = rk_bounds.as<uint32_t>();
+            d.t = teacher;
+            d.inv_t = teacher_inv_t;
+            d.sms = static_cast<uint32_t>(sms);
+            d.grad = r.grad;
+            d.hess = r.hess;
+            d.row_weight = r.weight;
+        }
         return r;
     }
 
@@ -253,6 +272,11 @@ struct sb2_backend {
 
     int check_loaded() {
         if (!loaded) return fail(SB2_EDEVICE, "b200 backend used before load");
+        return SB2_OK;
+    }
+    int check_teacher() {
+        if (objective.kind == SB2_DISTILL && teacher.top == 0)
+            return fail(SB2_ECONFIG, "the distillation objective has no teacher (sb2_set_teacher)");
         return SB2_OK;
     }
     int check_range(sb2_leaf_range leaf) {
@@ -480,6 +504,33 @@ std::vector<double> label_gains(const double* gain, uint32_t count) {
     return g;
 }
 
+// The dataset's query boundaries, checked; *longest (may be null) gets the most rows of a query.
+int check_queries(sb2_backend* b, const sb2_dataset* d, uint32_t* longest) {
+    const uint64_t n = d->num_rows;
+    const uint32_t nq = d->num_queries;
+    const uint32_t* qb = d->query_boundaries;
+    if (qb == nullptr || nq == 0) return b->fail(SB2_EDATA, "ranking tasks require query information");
+    if (qb[0] != 0 || qb[nq] != n) return b->fail(SB2_EDATA, "query boundaries must run from row 0 to the last row");
+    uint32_t most = 0;
+    for (uint32_t q = 0; q < nq; ++q) {
+        if (qb[q + 1] < qb[q]) return b->fail(SB2_EDATA, "query boundaries must not decrease");
+        most = std::max(most, qb[q + 1] - qb[q]);
+    }
+    if (longest) *longest = most;
+    return SB2_OK;
+}
+
+// The distillation objective's queries (its teacher comes with sb2_set_teacher).
+int load_distillation(sb2_backend* b, const sb2_dataset* d) {
+    SB2_TRY(check_queries(b, d, nullptr));
+    const uint32_t* qb = d->query_boundaries;
+    b->queries.assign(qb, qb + d->num_queries + 1);
+    SB2_CUDA(b, b->rk_bounds.alloc(sizeof(uint32_t) * b->queries.size()));
+    SB2_CUDA(b, cudaMemcpyAsync(b->rk_bounds.ptr, b->queries.data(), sizeof(uint32_t) * b->queries.size(),
+                                cudaMemcpyHostToDevice, b->stream));
+    return b->sync();
+}
+
 // ObjectiveSetup::LambdaRank (objective/mod.rs:35-65) for the device: the queries checked and uploaded, and the
 // tables the gradient kernel reads, computed here once with the reference's own expressions and the same libm
 // (lambdarank.rs:37-46 discounts, :51-72 the sigmoid table, :122-139 max DCG, :173-195 the label checks).
@@ -487,13 +538,8 @@ int load_ranking(sb2_backend* b, const sb2_dataset* d, const sb2_objective* o) {
     const uint64_t n = d->num_rows;
     const uint32_t nq = d->num_queries;
     const uint32_t* qb = d->query_boundaries;
-    if (qb == nullptr || nq == 0) return b->fail(SB2_EDATA, "ranking tasks require query information");
-    if (qb[0] != 0 || qb[nq] != n) return b->fail(SB2_EDATA, "query boundaries must run from row 0 to the last row");
     uint32_t longest = 0;
-    for (uint32_t q = 0; q < nq; ++q) {
-        if (qb[q + 1] < qb[q]) return b->fail(SB2_EDATA, "query boundaries must not decrease");
-        longest = std::max(longest, qb[q + 1] - qb[q]);
-    }
+    SB2_TRY(check_queries(b, d, &longest));
     if (longest > kMaxQueryRows)
         return b->fail(SB2_EUNSUPPORTED, "a query of " + std::to_string(longest) + " rows; the device takes " +
                                              std::to_string(kMaxQueryRows) + " at most");
@@ -591,10 +637,13 @@ int sb2_load(sb2_backend* b, const sb2_dataset* train, const sb2_objective* obje
     SB2_CUDA(b, cudaSetDevice(b->device));
     if (train->num_rows > 0xFFFFFFFFull)
         return b->fail(SB2_EUNSUPPORTED, std::to_string(train->num_rows) + " rows on one rank; the limit is 2^32 - 1");
-    if (objective->kind != SB2_REGRESSION && objective->kind != SB2_BINARY && objective->kind != SB2_LAMBDARANK)
+    if (objective->kind != SB2_REGRESSION && objective->kind != SB2_BINARY && objective->kind != SB2_LAMBDARANK &&
+        objective->kind != SB2_DISTILL)
         return b->fail(SB2_EUNSUPPORTED, "objective " + std::to_string(objective->kind) + " has no device gradients");
     b->ranking = RankArgs{};
+    b->teacher = TeacherArgs{};
     if (objective->kind == SB2_LAMBDARANK) SB2_TRY(load_ranking(b, train, objective));
+    if (objective->kind == SB2_DISTILL) SB2_TRY(load_distillation(b, train));
     const uint32_t F = train->num_features;
     b->features.assign(train->features, train->features + F);
     b->upper_bounds.assign(F, {});
@@ -997,6 +1046,7 @@ int sb2_init_scores(sb2_backend* b, int dataset, double value) {
 
 int sb2_compute_gradients(sb2_backend* b, sb2_gradient_stats* out) {
     SB2_TRY(b->check_loaded());
+    SB2_TRY(b->check_teacher());
     SB2_CUDA(b, cudaMemsetAsync(b->maxima.ptr, 0, 2 * sizeof(unsigned long long), b->stream));
     launch_api_gradients(b->row_args(), b->maxima.as<unsigned long long>(), b->row_grid(), b->stream);
     SB2_CUDA(b, cudaGetLastError());
@@ -1678,6 +1728,7 @@ int setup_training(sb2_backend* b, const sb2_params* p, double init_score, Train
          p->lambdarank_truncation_level != b->objective.lambdarank_truncation_level ||
          label_gains(p->label_gain, p->num_label_gain) != b->rank_gain))
         return b->fail(SB2_ECONFIG, "lambdarank parameters differ from the loaded objective's");
+    SB2_TRY(b->check_teacher());
     if (!p->use_quantized_grad) return b->fail(SB2_EUNSUPPORTED, "the device trainer is quantized only");
     if (p->bagging_fraction < 1.0 && p->bagging_freq > 0)
         return b->fail(SB2_EUNSUPPORTED, "bagging in the device trainer");
@@ -1932,7 +1983,7 @@ int sb2_train(sb2_backend* b, const sb2_params* p, double init_score, sb2_model*
 int sb2_boost_from_average(const sb2_params* p, const float* label, const float* weight, size_t n, double* out) {
     const double k_epsilon = static_cast<double>(1e-15f);
     *out = 0.0;
-    if (!p->boost_from_average || p->objective == SB2_LAMBDARANK) return SB2_OK;
+    if (!p->boost_from_average || p->objective == SB2_LAMBDARANK || p->objective == SB2_DISTILL) return SB2_OK;
     for (size_t i = 0; i < n; ++i)
         if (!std::isfinite(label[i])) {
             g_global_error = "label of row " + std::to_string(i) + " is not finite";
@@ -2183,6 +2234,239 @@ int sb2_bin_dense(sb2_backend* b, const void* values, int value_bytes, uint64_t 
         }
     }
     return b->sync();
+}
+
+}  // extern "C"
+
+namespace {
+
+// The handle's device for the length of a call; the caller's current device comes back after it.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t status;
+    explicit DeviceScope(int device) {
+        status = cudaGetDevice(&before);
+        if (status != cudaSuccess || before == device)
+            before = -1;
+        else
+            status = cudaSetDevice(device);
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Memory that a kernel of the handle's device may use: its device's own, or managed.
+int check_memory(sb2_backend* b, const void* p, const char* what) {
+    if (!p) return b->fail(SB2_EDATA, std::string(what) + " is null");
+    cudaPointerAttributes attr{};
+    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+        cudaGetLastError();
+        return b->fail(SB2_EDATA, std::string(what) + " is no device memory");
+    }
+    if (attr.type == cudaMemoryTypeManaged) return SB2_OK;
+    if (attr.type != cudaMemoryTypeDevice) return b->fail(SB2_EDATA, std::string(what) + " is no device memory");
+    if (attr.device != b->device)
+        return b->fail(SB2_EDATA, std::string(what) + " is memory of device " + std::to_string(attr.device) +
+                                      ", not of the handle's device " + std::to_string(b->device));
+    return SB2_OK;
+}
+
+int check_optional(sb2_backend* b, const void* p, const char* what) { return p ? check_memory(b, p, what) : SB2_OK; }
+
+uint64_t type_bytes(int32_t type) { return type == SB2_F32 ? 4 : 2; }
+
+int check_type(sb2_backend* b, int32_t type, const void* p, const char* what) {
+    if (type != SB2_F32 && type != SB2_BF16 && type != SB2_F16)
+        return b->fail(SB2_EDATA, std::string(what) + " of unknown type " + std::to_string(type));
+    if (reinterpret_cast<uintptr_t>(p) % type_bytes(type) != 0)
+        return b->fail(SB2_EDATA, std::string(what) + " are not aligned to their type");
+    return SB2_OK;
+}
+
+int check_temperature(sb2_backend* b, double temperature) {
+    if (!(temperature >= 1e-6 && temperature <= 1e6))
+        return b->fail(SB2_ECONFIG, "the temperature must be between 1e-6 and 1e6");
+    return SB2_OK;
+}
+
+int list_args(sb2_backend* b, const sb2_lists* lists, ListsArgs& a) {
+    constexpr uint64_t kMost = 1ull << 60;  // entries: no offset in bytes passes 64 bits
+    SB2_TRY(check_type(b, lists->type, lists->scores_dev, "the scores"));
+    if (lists->boundaries_dev == nullptr) {
+        if (lists->width > 0x7FFFFFFFull)
+            return b->fail(SB2_EUNSUPPORTED, "lists of " + std::to_string(lists->width) + " entries; the limit is 2^31 - 1");
+        if (lists->num_lists > 1 && lists->stride < lists->width)
+            return b->fail(SB2_EDATA, "lists of " + std::to_string(lists->width) + " entries, " +
+                                          std::to_string(lists->stride) + " from one to the next");
+        if (lists->num_lists > 1 && lists->stride > kMost / lists->num_lists)
+            return b->fail(SB2_EUNSUPPORTED, "a stride of " + std::to_string(lists->stride) + " entries");
+    } else {
+        if (lists->width > 0xFFFFFFFFull)
+            return b->fail(SB2_EUNSUPPORTED, std::to_string(lists->width) + " entries behind boundaries; the limit is 2^32 - 1");
+        SB2_TRY(check_memory(b, lists->boundaries_dev, "the boundaries"));
+    }
+    if (lists->num_lists > 0 && lists->width > 0) SB2_TRY(check_memory(b, lists->scores_dev, "the scores"));
+    a.scores = lists->scores_dev;
+    a.type = lists->type;
+    a.lists = lists->num_lists;
+    a.width = lists->width;
+    a.stride = lists->stride;
+    a.bounds = lists->boundaries_dev;
+    return SB2_OK;
+}
+
+// Bytes from a list array's first entry to behind its last.
+uint64_t extent(const ListsArgs& l, uint64_t stride) {
+    const uint64_t entries = l.bounds != nullptr ? l.width : l.lists == 0 ? 0 : (l.lists - 1ull) * stride + l.width;
+    return entries * type_bytes(l.type);
+}
+
+bool overlap(const void* p, uint64_t bytes_p, const void* q, uint64_t bytes_q) {
+    const uint64_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return a < b + bytes_q && b < a + bytes_p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sb2_log_probs(sb2_backend* b, const sb2_lists* lists, double temperature, const int32_t* given_dev,
+                  uint32_t num_given, uint32_t top, float* given_out_dev, float* entropy_dev, float* log_sum_dev,
+                  int32_t* top_ids_dev, float* top_out_dev, void* stream) {
+    if (!b) return SB2_EDEVICE;
+    if (!lists) return b->fail(SB2_EDATA, "no lists");
+    const DeviceScope scope(b->device);
+    SB2_CUDA(b, scope.status);
+    SB2_TRY(check_temperature(b, temperature));
+    if (top > kMaxTop)
+        return b->fail(SB2_EUNSUPPORTED, std::to_string(top) + " alternatives; the limit is " + std::to_string(kMaxTop));
+    LogProbsArgs a{};
+    SB2_TRY(list_args(b, lists, a.l));
+    if (a.l.lists == 0) return SB2_OK;
+    if (num_given > 0) {
+        SB2_TRY(check_memory(b, given_dev, "the given entries"));
+        SB2_TRY(check_memory(b, given_out_dev, "the given entries' output"));
+    }
+    if (top > 0) {
+        SB2_TRY(check_memory(b, top_ids_dev, "the alternatives' indices"));
+        SB2_TRY(check_memory(b, top_out_dev, "the alternatives' output"));
+    }
+    SB2_TRY(check_optional(b, entropy_dev, "the entropy"));
+    SB2_TRY(check_optional(b, log_sum_dev, "the log sums"));
+    a.inv_t = static_cast<float>(1.0 / temperature);
+    a.sms = static_cast<uint32_t>(b->sms);
+    a.num_given = num_given;
+    a.top = top;
+    a.given = given_dev;
+    a.given_out = given_out_dev;
+    a.entropy = entropy_dev;
+    a.log_sum = log_sum_dev;
+    a.top_ids = top_ids_dev;
+    a.top_out = top_out_dev;
+    launch_log_probs(a, static_cast<cudaStream_t>(stream));
+    return b->cuda(cudaGetLastError(), "sb2_log_probs");
+}
+
+int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* teacher, double temperature,
+                const float* weight_dev, float* loss_dev, void* grad_dev, void* hess_dev, uint64_t grad_stride,
+                void* stream) {
+    if (!b) return SB2_EDEVICE;
+    if (!student || !teacher) return b->fail(SB2_EDATA, "no student or no teacher");
+    const DeviceScope scope(b->device);
+    SB2_CUDA(b, scope.status);
+    SB2_TRY(check_temperature(b, temperature));
+    if (teacher->top < 1 || teacher->top > kMaxTop)
+        return b->fail(SB2_EUNSUPPORTED, "a teacher's top of " + std::to_string(teacher->top) + " entries; 1 to " +
+                                             std::to_string(kMaxTop) + " are taken");
+    if (teacher->stride < teacher->top || teacher->stride > (1ull << 28))
+        return b->fail(SB2_EDATA, "a teacher's top of " + std::to_string(teacher->top) + " entries, " +
+                                      std::to_string(teacher->stride) + " from one list to the next");
+    DistillArgs a{};
+    SB2_TRY(list_args(b, student, a.l));
+    if (a.l.lists == 0) return SB2_OK;
+    SB2_TRY(check_type(b, teacher->type, teacher->logits_dev, "the teacher's logits"));
+    SB2_TRY(check_memory(b, teacher->ids_dev, "the teacher's ids"));
+    SB2_TRY(check_memory(b, teacher->logits_dev, "the teacher's logits"));
+    SB2_TRY(check_optional(b, teacher->log_sum_dev, "the teacher's log sums"));
+    SB2_TRY(check_optional(b, weight_dev, "the weights"));
+    SB2_TRY(check_optional(b, loss_dev, "the loss"));
+    if (grad_stride == 0) grad_stride = student->stride;
+    if (a.l.bounds == nullptr && a.l.lists > 1 && (grad_dev || hess_dev) &&
+        (grad_stride < a.l.width || grad_stride > (1ull << 60) / a.l.lists))
+        return b->fail(SB2_EDATA, "gradients of " + std::to_string(a.l.width) + " entries, " + std::to_string(grad_stride) +
+                                      " from one list to the next");
+    for (const void* out : {static_cast<const void*>(grad_dev), static_cast<const void*>(hess_dev)}) {
+        if (!out || a.l.width == 0) continue;
+        SB2_TRY(check_type(b, a.l.type, out, "the gradients"));
+        SB2_TRY(check_memory(b, out, "the gradients"));
+        if (overlap(a.l.scores, extent(a.l, a.l.stride), out, extent(a.l, grad_stride)))
+            return b->fail(SB2_EDATA, "the gradients overlap the scores");
+    }
+    if (grad_dev && hess_dev && overlap(grad_dev, extent(a.l, grad_stride), hess_dev, extent(a.l, grad_stride)))
+        return b->fail(SB2_EDATA, "gradient and hessian overlap");
+    a.t.ids = teacher->ids_dev;
+    a.t.logits = teacher->logits_dev;
+    a.t.log_sum = teacher->log_sum_dev;
+    a.t.type = teacher->type;
+    a.t.top = teacher->top;
+    a.t.stride = teacher->stride;
+    a.inv_t = static_cast<float>(1.0 / temperature);
+    a.sms = static_cast<uint32_t>(b->sms);
+    a.grad_stride = grad_stride;
+    a.weight = weight_dev;
+    a.loss = loss_dev;
+    a.grad = grad_dev;
+    a.hess = hess_dev;
+    launch_distill(a, static_cast<cudaStream_t>(stream));
+    return b->cuda(cudaGetLastError(), "sb2_distill");
+}
+
+int sb2_set_teacher(sb2_backend* b, const int32_t* ids, const float* logits, const float* log_sum, uint64_t num_lists,
+                    uint32_t top, double temperature) {
+    if (!b) return SB2_EDEVICE;
+    SB2_TRY(b->check_loaded());
+    if (b->objective.kind != SB2_DISTILL)
+        return b->fail(SB2_ECONFIG, "a teacher for another objective than the distillation's");
+    SB2_TRY(check_temperature(b, temperature));
+    if (top < 1 || top > kMaxTop)
+        return b->fail(SB2_EUNSUPPORTED, "a teacher's top of " + std::to_string(top) + " entries; 1 to " +
+                                             std::to_string(kMaxTop) + " are taken");
+    const uint64_t nq = b->queries.size() - 1;
+    if (num_lists != nq)
+        return b->fail(SB2_EDATA, "a teacher of " + std::to_string(num_lists) + " lists for " + std::to_string(nq) + " queries");
+    if (!ids || !logits) return b->fail(SB2_EDATA, "the teacher's ids or logits are null");
+    for (uint64_t q = 0; q < nq; ++q) {
+        const int64_t rows = static_cast<int64_t>(b->queries[q + 1]) - b->queries[q];
+        for (uint64_t e = q * top; e < (q + 1) * top; ++e) {
+            if (ids[e] == -1) continue;
+            if (ids[e] < 0 || ids[e] >= rows)
+                return b->fail(SB2_EDATA, "the teacher names row " + std::to_string(ids[e]) + " of query " +
+                                              std::to_string(q) + ", which has " + std::to_string(rows));
+            if (!(logits[e] < std::numeric_limits<float>::infinity()))
+                return b->fail(SB2_EDATA, "a teacher's logit of query " + std::to_string(q) + " is NaN or infinite");
+        }
+        if (log_sum && !std::isfinite(log_sum[q]))
+            return b->fail(SB2_EDATA, "the teacher's log sum of query " + std::to_string(q) + " is not finite");
+    }
+    SB2_CUDA(b, cudaSetDevice(b->device));
+    b->teacher = TeacherArgs{};  // none while the buffers change
+    SB2_CUDA(b, b->teach_ids.alloc(sizeof(int32_t) * nq * top));
+    SB2_CUDA(b, b->teach_logits.alloc(sizeof(float) * nq * top));
+    SB2_CUDA(b, b->teach_log_sum.alloc(sizeof(float) * (log_sum ? nq : 0)));
+    SB2_CUDA(b, cudaMemcpyAsync(b->teach_ids.ptr, ids, sizeof(int32_t) * nq * top, cudaMemcpyHostToDevice, b->stream));
+    SB2_CUDA(b, cudaMemcpyAsync(b->teach_logits.ptr, logits, sizeof(float) * nq * top, cudaMemcpyHostToDevice, b->stream));
+    if (log_sum)
+        SB2_CUDA(b, cudaMemcpyAsync(b->teach_log_sum.ptr, log_sum, sizeof(float) * nq, cudaMemcpyHostToDevice, b->stream));
+    SB2_TRY(b->sync());
+    b->teacher.ids = b->teach_ids.as<int32_t>();
+    b->teacher.logits = b->teach_logits.as<float>();
+    b->teacher.log_sum = log_sum ? b->teach_log_sum.as<float>() : nullptr;
+    b->teacher.type = SB2_F32;
+    b->teacher.top = top;
+    b->teacher.stride = top;
+    b->teacher_inv_t = static_cast<float>(1.0 / temperature);
+    return SB2_OK;
 }
 
 int sb2_model_free(sb2_model* m) {

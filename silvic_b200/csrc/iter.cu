@@ -729,11 +729,24 @@ __global__ void division_check_kernel(uint64_t n, uint32_t seed, unsigned long l
     if (bad) atomicAdd(mismatches, bad);
 }
 
+// The distillation objective's gradients and their maxima; nothing when `stopped` (may be null) is set. Launch errors
+// surface at the caller's cudaGetLastError, as the other launches'.
+void launch_teacher(const RowArgs& r, const int32_t* stopped, unsigned long long* max_g, unsigned long long* max_h,
+                    cudaStream_t s) {
+    DistillArgs d = r.distill;
+    d.stopped = stopped;
+    d.max_g = max_g;
+    d.max_h = max_h;
+    launch_distill(d, s);
+}
+
 }  // namespace
 
 void launch_gradients(const IterArgs& a, int grid, cudaStream_t s) {
     if (a.r.objective == SB2_LAMBDARANK)
         launch_lambdarank(a.r, &a.t.iter->stopped, &a.t.iter->max_abs_grad_bits, &a.t.iter->max_hess_bits, s);
+    else if (a.r.objective == SB2_DISTILL)
+        launch_teacher(a.r, &a.t.iter->stopped, &a.t.iter->max_abs_grad_bits, &a.t.iter->max_hess_bits, s);
     else
         gradients_kernel<<<grid, kRowThreads, 0, s>>>(a);
 }
@@ -753,6 +766,8 @@ void launch_add_tree_partition(const IterArgs& a, int grid, cudaStream_t s) {
 void launch_api_gradients(const RowArgs& r, unsigned long long* bits, int grid, cudaStream_t s) {
     if (r.objective == SB2_LAMBDARANK)
         launch_lambdarank(r, nullptr, bits, bits + 1, s);
+    else if (r.objective == SB2_DISTILL)
+        launch_teacher(r, nullptr, bits, bits + 1, s);
     else
         api_gradients_kernel<<<grid, kRowThreads, 0, s>>>(r, bits);
 }

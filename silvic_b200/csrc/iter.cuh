@@ -1,6 +1,7 @@
 // iter.cuh — per-iteration kernels of the boosting loop (boosting.rs:227-324) and the Backend-API kernels.
 #pragma once
 
+#include "lists.cuh"
 #include "train.cuh"
 
 namespace sb2 {
@@ -31,7 +32,7 @@ struct RankArgs {
 struct RowArgs {
     uint64_t num_rows;
     uint64_t row_offset;
-    int32_t objective;   // SB2_REGRESSION / SB2_BINARY / SB2_LAMBDARANK
+    int32_t objective;   // SB2_REGRESSION / SB2_BINARY / SB2_LAMBDARANK / SB2_DISTILL
     int32_t pad_;
     double sigmoid;
     const float* label;
@@ -41,6 +42,7 @@ struct RowArgs {
     float* hess;
     int32_t* packed;
     RankArgs rank;        // lambdarank only
+    DistillArgs distill;  // distillation only: the queries' scores as lists, the teacher, grad and hess
 };
 
 // Training constants of one run (Params subset) the iteration kernels need.

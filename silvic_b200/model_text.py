@@ -402,7 +402,8 @@ def model_parameters(params: _abi.Params) -> list:
     """`Params::model_parameters` (config.rs:444-498) for the parameters a device-trained model carries (lambdarank's
     three after the quantization ones, config.rs:486-493); the binning parameters the device trainer does not take
     keep the reference's defaults (config.rs:123-167)."""
-    objective = {_abi.REGRESSION: "regression", _abi.BINARY: "binary"}.get(params.objective, "lambdarank")
+    objective = {_abi.REGRESSION: "regression", _abi.BINARY: "binary", _abi.DISTILL: "custom"}.get(params.objective,
+                                                                                               "lambdarank")
     g = format_g
     out = [("boosting", "gbdt"), ("objective", objective), ("num_iterations", str(params.num_iterations)),
            ("learning_rate", g(params.learning_rate)), ("num_leaves", str(params.num_leaves)),
@@ -428,7 +429,7 @@ def model_parameters(params: _abi.Params) -> list:
         out += [("lambdarank_truncation_level", str(params.lambdarank_truncation_level)),
                 ("lambdarank_norm", str(int(bool(params.lambdarank_norm)))),
                 ("label_gain", ",".join(g(v) for v in gains))]
-    if objective != "regression":
+    if objective not in ("regression", "custom"):
         out.append(("sigmoid", g(params.sigmoid)))
     return out
 
@@ -472,7 +473,8 @@ def _categorical_splits(tr, n: int, dataset):
 def from_trained(model, dataset, params: _abi.Params) -> TextModel:
     """A device- (or oracle-) trained model (`silvic_b200.backend.Model`) as silvic's model file of the same
     training run (`boosting::train_from`, boosting.rs:151-190): feature names and infos from the dataset's features,
-    the parameters of `params`."""
+    the parameters of `params`. A distilled model's objective line says lambdarank: its scores are a ranker's raw
+    scores, and the format's readers take no objective that they do not know; its parameters say custom."""
     objective = {_abi.REGRESSION: "regression", _abi.BINARY: "binary"}.get(params.objective, "lambdarank")
     trees = []
     for tr in model.trees:
