@@ -426,7 +426,7 @@ typedef struct sb2_lists {
     const void* scores_dev;
     int32_t type;                   /* of the scores: SB2_F32 / SB2_BF16 / SB2_F16 */
     uint32_t num_lists;
-    uint64_t width;                 /* dense: entries of a list (below 2^31); with boundaries: entries behind scores_dev */
+    uint64_t width;                 /* dense: entries of a list; with boundaries: entries behind scores_dev; below 2^31 */
     uint64_t stride;                /* dense: entries from one list to the next (at least width for 2 lists and more) */
     const uint32_t* boundaries_dev; /* NULL: dense; else num_lists + 1 boundaries that do not decrease (what lies
                                        outside the entries is cut off), as sb2_dataset's query_boundaries */

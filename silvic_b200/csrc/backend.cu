@@ -504,7 +504,7 @@ std::vector<double> label_gains(const double* gain, uint32_t count) {
     return g;
 }
 
-// The dataset's query boundaries, checked; *longest (may be null) gets the most rows of a query.
+// The dataset's query boundaries, checked; *longest gets the most rows of a query.
 int check_queries(sb2_backend* b, const sb2_dataset* d, uint32_t* longest) {
     const uint64_t n = d->num_rows;
     const uint32_t nq = d->num_queries;
@@ -516,13 +516,15 @@ int check_queries(sb2_backend* b, const sb2_dataset* d, uint32_t* longest) {
         if (qb[q + 1] < qb[q]) return b->fail(SB2_EDATA, "query boundaries must not decrease");
         most = std::max(most, qb[q + 1] - qb[q]);
     }
-    if (longest) *longest = most;
+    *longest = most;
     return SB2_OK;
 }
 
 // The distillation objective's queries (its teacher comes with sb2_set_teacher).
 int load_distillation(sb2_backend* b, const sb2_dataset* d) {
-    SB2_TRY(check_queries(b, d, nullptr));
+    uint32_t longest = 0;
+    SB2_TRY(check_queries(b, d, &longest));
+    if (longest > 0x7FFFFFFFu) return b->fail(SB2_EUNSUPPORTED, "a query of 2^31 rows and more");
     const uint32_t* qb = d->query_boundaries;
     b->queries.assign(qb, qb + d->num_queries + 1);
     SB2_CUDA(b, b->rk_bounds.alloc(sizeof(uint32_t) * b->queries.size()));
@@ -2302,8 +2304,8 @@ int list_args(sb2_backend* b, const sb2_lists* lists, ListsArgs& a) {
         if (lists->num_lists > 1 && lists->stride > kMost / lists->num_lists)
             return b->fail(SB2_EUNSUPPORTED, "a stride of " + std::to_string(lists->stride) + " entries");
     } else {
-        if (lists->width > 0xFFFFFFFFull)
-            return b->fail(SB2_EUNSUPPORTED, std::to_string(lists->width) + " entries behind boundaries; the limit is 2^32 - 1");
+        if (lists->width > 0x7FFFFFFFull)
+            return b->fail(SB2_EUNSUPPORTED, std::to_string(lists->width) + " entries behind boundaries; the limit is 2^31 - 1");
         SB2_TRY(check_memory(b, lists->boundaries_dev, "the boundaries"));
     }
     if (lists->num_lists > 0 && lists->width > 0) SB2_TRY(check_memory(b, lists->scores_dev, "the scores"));

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a) {
         if (m == -CUDART_INF_F) m = 0.0f;
         float in = 0.0f, out = 0.0f;
         for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-            const float e = exp_of(__fsub_rn(to_float(z[j]), m), c);
+            const float e = pow2(exponent(to_float(z[j]), m, c));
             bool taught = false;
             for (uint32_t t = 0; rest && t < k; ++t) taught |= s_id[t] == static_cast<int32_t>(j);
             if (taught)
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a) {
         if (threadIdx.x == 0 && a.loss != nullptr) a.loss[i] = empty ? 0.0f : loss * w;
         const uint64_t to = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
         for (uint32_t j = threadIdx.x; j < n && (a.grad != nullptr || a.hess != nullptr); j += kThreads) {
-            const float p = empty ? 0.0f : exp_of(__fsub_rn(to_float(z[j]), m), c) * inv_s;
+            const float p = empty ? 0.0f : pow2(exponent(to_float(z[j]), m, c)) * inv_s;
             float teach = 0.0f;
             bool taught = false;
             for (uint32_t t = 0; t < k; ++t)

@@ -60,6 +60,14 @@ struct DistillArgs {
     unsigned long long* max_h;
 };
 
+// CTAs that share a list of `entries`, as a cluster: while the lists leave half of the SMs without a CTA and a share
+// keeps 4096 entries, twice as many, 8 at most (the largest cluster every device of the architecture takes).
+inline uint32_t list_shares(uint64_t entries, uint32_t lists, uint32_t sms) {
+    uint32_t shares = 1;
+    while (shares < 8 && static_cast<uint64_t>(lists) * shares * 2 <= 2 * sms && entries / (2 * shares) >= 4096) shares *= 2;
+    return shares;
+}
+
 // One launch each; errors are left for the caller's cudaGetLastError.
 void launch_log_probs(const LogProbsArgs& a, cudaStream_t s);
 void launch_distill(const DistillArgs& a, cudaStream_t s);

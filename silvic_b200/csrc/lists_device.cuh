@@ -1,6 +1,7 @@
 // lists_device.cuh — what the kernels over lists of candidates share on the device.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -11,6 +12,7 @@
 namespace sb2 {
 
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr uint32_t kFull = 0xffffffffu;
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -48,15 +50,104 @@ __device__ __forceinline__ void list_range(const ListsArgs& l, uint32_t i, uint6
 }
 
 // The order of alternatives as one ascending key: the score (-0 as 0, NaN above everything), then the lower index.
-__device__ __forceinline__ unsigned long long order_key(float z, uint32_t index) {
+__device__ __forceinline__ uint32_t order_of(float z) {
     const uint32_t bits = __float_as_uint(__fadd_rn(z, 0.0f));
-    uint32_t order = (bits >> 31) != 0 ? ~bits : (bits | 0x80000000u);
-    if (z != z) order = 0xFFFFFFFFu;
-    return (static_cast<unsigned long long>(order) << 32) | (0xFFFFFFFFu - index);
+    return z != z ? 0xFFFFFFFFu : (bits >> 31) != 0 ? ~bits : (bits | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long order_key(float z, uint32_t index) {
+    return (static_cast<unsigned long long>(order_of(z)) << 32) | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ uint32_t index_of(unsigned long long key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
+
+// 2^x, at most 2 ulp off (ex2.approx); results below 2^-126 are 0.
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// exp((z - m) / T) with c = log2(e) / T: the difference first, so the argument's error grows with the distance from
-// the maximum, where the terms are small, and not with the scores' size.
-__device__ __forceinline__ float exp_of(float d, float c) { return exp2f(__fmul_rn(d, c)); }
+// max that keeps a NaN of either side.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// exp((z - m) / T) is pow2(y) with y = exponent(z - m, c), c = log2(e) / T: the difference first, so the argument's
+// error grows with the distance from the reference, where the terms are small, and not with the scores' size. A masked
+// score's exponent is finite, so that 0 times it is 0.
+__device__ __forceinline__ float exponent(float z, float m, float c) { return max_nan(__fmul_rn(__fsub_rn(z, m), c), -200.0f); }
+
+// A list as one thread block (or a cluster of them) walks it: scalars up to the first 16-byte boundary, vectors of
+// kVec entries, scalars behind the last. kVec 1: entry by entry, so that sums do not depend on where a list starts.
+template <class T, int kVec>
+struct Walk {
+    const T* z;
+    uint32_t n, head, vectors;
+    __device__ __forceinline__ Walk(const T* scores, uint32_t entries) : z(scores), n(entries) {
+        head = 0;
+        if (kVec > 1) head = min(n, static_cast<uint32_t>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / static_cast<uint32_t>(sizeof(T)));
+        vectors = (n - head) / kVec;
+    }
+    // The first entry of vector v, and where the scalars behind the vectors start.
+    __device__ __forceinline__ uint32_t at(uint32_t v) const { return head + v * kVec; }
+    __device__ __forceinline__ uint32_t tail() const { return head + vectors * kVec; }
+    // Scalars outside the vectors, fewer than 2 kVec: entry of scalar i, or n behind the last.
+    __device__ __forceinline__ uint32_t edge(uint32_t i) const {
+        if (i < head) return i;
+        const uint32_t j = tail() + (i - head);
+        return j < n ? j : n;
+    }
+};
+
+// The packed entries of one vector.
+template <class T, int kVec>
+struct Pack {
+    uint4 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void values(float (&f)[kVec]) const {
+        if constexpr (sizeof(T) == 4) {
+            f[0] = __uint_as_float(raw.x);
+            f[1] = __uint_as_float(raw.y);
+            f[2] = __uint_as_float(raw.z);
+            f[3] = __uint_as_float(raw.w);
+        } else {
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                    f[2 * i] = __uint_as_float(w[i] << 16);
+                    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                } else {
+                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    f[2 * i] = v.x;
+                    f[2 * i + 1] = v.y;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void masked() {  // every entry -inf
+        const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, __nv_bfloat16> ? 0xFF80FF80u : 0xFC00FC00u;
+        raw = make_uint4(w, w, w, w);
+    }
+};
+template <class T>
+struct Pack<T, 1> {
+    T raw;
+    __device__ __forceinline__ void load(const T* p) { raw = __ldg(p); }
+    __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = to_float(raw); }
+    __device__ __forceinline__ void masked() { raw = from_float<T>(-CUDART_INF_F); }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
 
 }  // namespace sb2

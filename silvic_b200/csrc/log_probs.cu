@@ -1,111 +1,513 @@
 // log_probs.cu — log probabilities of given entries, entropy and top alternatives of softmax(z / T) over each list.
 //
-// With m = max z, S = sum exp((z - m) / T) and U = sum exp((z - m) / T) (z - m):
-//   log p_i = (z_i - m) / T - ln S,  log sum = m / T + ln S,  entropy = ln S - U / (T S).
-// Statistics are f32 sums; the alternatives are ordered by the scores themselves (ties by the lower index), so no
-// rounding decides an index.
+// With a reference m near max z, y_j = (z_j - m) log2(e) / T, S = sum 2^y and V = sum 2^y y:
+//   log p_j = (z_j - m) / T - ln S,  log sum = m / T + ln S,  entropy = ln S - ln 2 V / S.
+// Statistics are f32 sums over one pass; the alternatives are ordered by the scores themselves (ties by the lower
+// index), so no rounding decides an index.
+//
+// Lists of at most kWarpEntries take a warp each, in registers. Longer ones take a CTA (few of them: a cluster of
+// CTAs), which reads the list once: the maxima of the first batch give the reference, a bound that at least `top`
+// entries reach, and so a filter; entries that pass it are gathered in shared memory and ranked at the end. A list
+// whose order defeats the filter (more candidates than the buffer holds) has its alternatives selected again, digit by
+// digit of their keys.
+#include <cfloat>
+
 #include "lists_device.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace sb2 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr uint32_t kWarpEntries = 512;
+constexpr int kWarpThreads = 256;        // the warp kernel's CTAs
+constexpr uint32_t kCandidates = 2048;   // keys that a CTA gathers
+constexpr int kBatch = 4;                // vectors a thread holds in flight
+constexpr float kSlack = 4.0f;           // log2 units that an entry may lie above the reference before it moves
 
-// The block's maximum of a key, in every thread.
-__device__ __forceinline__ unsigned long long block_max_key(unsigned long long k, unsigned long long* s) {
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-        k = k > other ? k : other;
+struct Stats {
+    float m, s, v;  // the reference, the sum of 2^y, the sum of 2^y y
+};
+
+// Statistics about another reference.
+__device__ __forceinline__ void rebase(Stats& a, float m, float c) {
+    const float y = exponent(a.m, m, c), f = pow2(y);
+    a.v = f * (a.v + a.s * y);
+    a.s *= f;
+    a.m = m;
+}
+
+// What a CTA keeps of its share of a list.
+template <int kThreads>
+struct Shared {
+    unsigned long long key[kCandidates];
+    unsigned long long best[kMaxTop];  // the share's alternatives, likeliest first; 0 behind the last
+    uint32_t order[256];               // group maxima, then the digits' counts
+    float warp[3][kThreads / 32];
+    Stats stats;
+    float bound;
+    uint32_t count, digit, left;
+};
+
+// The share's `top` largest keys of `count` gathered ones into s.best, in order. Few: every key counts the keys above
+// it; many: a bitonic sort. Ends without a barrier behind the writes of s.best.
+template <int kThreads>
+__device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t count, uint32_t top) {
+    const uint32_t t = threadIdx.x;
+    for (uint32_t i = t; i < top; i += kThreads) s.best[i] = 0;
+    __syncthreads();
+    if (count <= 512) {
+        for (uint32_t i = t; i < count; i += kThreads) {
+            const unsigned long long mine = s.key[i];
+            uint32_t above = 0;
+            for (uint32_t j = 0; j < count; ++j) above += s.key[j] > mine;
+            if (above < top) s.best[above] = mine;
+        }
+        return;
+    }
+    uint32_t cap = 1024;
+    while (cap < count) cap <<= 1;
+    for (uint32_t i = count + t; i < cap; i += kThreads) s.key[i] = 0;
+    __syncthreads();
+    for (uint32_t size = 2; size <= cap; size <<= 1)
+        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
+            for (uint32_t x = t; x < cap / 2; x += kThreads) {
+                const uint32_t lo = 2 * x - (x & (stride - 1)), hi = lo + stride;
+                const unsigned long long a = s.key[lo], b = s.key[hi];
+                if ((a < b) == ((lo & size) == 0)) {
+                    s.key[lo] = b;
+                    s.key[hi] = a;
+                }
+            }
+            __syncthreads();
+        }
+    for (uint32_t i = t; i < top; i += kThreads) s.best[i] = s.key[i];
+}
+
+// Entries [from, to) of the vectors and, for share 0, the scalars outside them, each to `f(score, index)`.
+template <class T, int kVec, int kThreads, class F>
+__device__ __forceinline__ void for_share(const Walk<T, kVec>& w, uint32_t from, uint32_t to, bool edges, F f) {
+    for (uint32_t v = from + threadIdx.x; v < to; v += kThreads) {
+        Pack<T, kVec> p;
+        p.load(w.z + w.at(v));
+        float x[kVec];
+        p.values(x);
+        for (int e = 0; e < kVec; ++e) f(x[e], w.at(v) + e);
+    }
+    if (edges) {
+        const uint32_t j = w.edge(threadIdx.x);
+        if (threadIdx.x < 2 * kVec && j < w.n) f(to_float(w.z[j]), j);
+    }
+}
+
+// The share's `top`-th largest key, digit by digit, then the keys from it on: exactly `top` candidates, whatever the
+// order or the ties. The share holds more unmasked entries than kCandidates.
+template <class T, int kVec, int kThreads>
+__device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, uint32_t n, uint32_t from, uint32_t to, bool edges,
+                                               uint32_t top) {
+    const Walk<T, kVec> w(z, n);
+    unsigned long long prefix = 0;
+    uint32_t left = top;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < 256; i += kThreads) s.order[i] = 0;
+        __syncthreads();
+        for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
+            const unsigned long long key = order_key(x, j);
+            if (x > -CUDART_INF_F && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
+                atomicAdd(&s.order[static_cast<uint32_t>(key >> shift) & 255u], 1u);
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t d = 255, need = left;
+            while (d > 0 && s.order[d] < need) need -= s.order[d--];
+            s.digit = d;
+            s.left = need;
+        }
+        __syncthreads();
+        prefix |= static_cast<unsigned long long>(s.digit) << shift;
+        left = s.left;
+    }
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
+        const unsigned long long key = order_key(x, j);
+        if (x > -CUDART_INF_F && key >= prefix) {
+            const uint32_t at = atomicAdd(&s.count, 1u);
+            if (at < kCandidates) s.key[at] = key;
+        }
+    });
+    __syncthreads();
+}
+
+// One thread's running statistics and its filter for alternatives.
+template <class T, int kVec, int kThreads>
+struct Reader {
+    Shared<kThreads>& s;
+    Stats a;
+    float c, limit, bound;
+
+    __device__ __forceinline__ void gather(float x, uint32_t j) {
+        if (x >= bound && x > -CUDART_INF_F) {
+            const uint32_t at = atomicAdd(&s.count, 1u);
+            if (at < kCandidates) s.key[at] = order_key(x, j);
+        }
+    }
+    template <int kCount>
+    __device__ __forceinline__ void add(const float (&x)[kCount], uint32_t first) {
+        float most = x[0];
+#pragma unroll
+        for (int e = 1; e < kCount; ++e) most = fmaxf(most, x[e]);
+        if (most > limit) {
+            rebase(a, most, c);
+            limit = most + kSlack / c;
+        }
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            const float y = exponent(x[e], a.m, c), p = pow2(y);
+            a.s += p;
+            a.v = __fmaf_rn(p, y, a.v);
+        }
+        if (most >= bound && s.count <= kCandidates) {
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) gather(x[e], first + e);
+        }
+    }
+};
+
+// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1).
+template <class T, int kVec, int kThreads, bool kCluster>
+__device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogProbsArgs& a, uint32_t i, uint32_t share,
+                                               uint32_t shares) {
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    uint64_t first;
+    uint32_t n;
+    list_range(a.l, i, first, n);
+    const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
+    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * share / shares);
+    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * (share + 1) / shares);
+    const float c = __fmul_rn(kLog2E, a.inv_t);
+    // The given entries' scores, on their way while the list is read.
+    float given = -CUDART_INF_F;
+    if (share == 0 && t < a.num_given) {
+        const int32_t id = a.given[static_cast<uint64_t>(i) * a.num_given + t];
+        if (id >= 0 && static_cast<uint32_t>(id) < n) given = to_float(w.z[id]);
+    }
+    // The first batch, and the scalars outside the vectors (share 0): their maximum.
+    Pack<T, kVec> p[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const uint32_t v = from + u * kThreads + t;
+        if (v < to)
+            p[u].load(w.z + w.at(v));
+        else
+            p[u].masked();
+    }
+    float edge[1] = {-CUDART_INF_F};
+    const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
+    if (edge_at < n) edge[0] = to_float(w.z[edge_at]);
+    float most = edge[0];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        float x[kVec];
+        p[u].values(x);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) most = fmaxf(most, x[e]);
+    }
+    // Groups of threads: `top` groups reach the top-th largest of their maxima, so `top` entries do.
+    const uint32_t groups = min(static_cast<uint32_t>(kThreads), a.top > 64 ? 256u : 128u), per = kThreads / groups;
+    float group = most;
+    for (uint32_t o = 1; o < per; o <<= 1) group = fmaxf(group, __shfl_xor_sync(kFull, group, o));
+    if (t % per == 0) s.order[t / per] = order_of(group);
+    most = warp_max(most);
+    if (lane == 0) s.warp[0][warp] = most;
+    if (t == 0) {
+        s.count = 0;
+        s.bound = -CUDART_INF_F;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = k;
+    most = s.warp[0][0];
+#pragma unroll
+    for (int k = 1; k < kThreads / 32; ++k) most = fmaxf(most, s.warp[0][k]);
+    if (a.top == 0) {
+        if (t == 0) s.bound = CUDART_INF_F;
+    } else if (t < groups) {
+        const uint32_t mine = s.order[t];
+        uint32_t above = 0;
+        for (uint32_t j = 0; j < groups; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(&s.order[j]);
+            above += (o.x > mine || (o.x == mine && j < t)) + (o.y > mine || (o.y == mine && j + 1 < t)) +
+                     (o.z > mine || (o.z == mine && j + 2 < t)) + (o.w > mine || (o.w == mine && j + 3 < t));
+        }
+        if (above == a.top - 1) s.bound = __uint_as_float((mine >> 31) != 0 ? mine & 0x7FFFFFFFu : ~mine);
+    }
     __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) k = k > s[w] ? k : s[w];
-    return k;
+    // One pass: the statistics about the first batch's maximum (moved where later entries lie far above it), and the
+    // entries that reach the bound.
+    Reader<T, kVec, kThreads> r{s, {most == -CUDART_INF_F ? -FLT_MAX : most, 0.0f, 0.0f}, c, 0.0f, s.bound};
+    r.limit = r.a.m + kSlack / c;
+    for (uint32_t v = from + t; v < to; v += kBatch * kThreads) {
+        Pack<T, kVec> now[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            now[u] = p[u];
+            const uint32_t next = v + (u + kBatch) * kThreads;
+            if (next < to) p[u].load(w.z + w.at(next));
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (v + u * kThreads < to) {
+                float x[kVec];
+                now[u].values(x);
+                r.add(x, w.at(v + u * kThreads));
+            }
+        }
+    }
+    if (edge_at < n) r.add(edge, edge_at);
+    // The share's statistics.
+    const float top_m = warp_max(r.a.m);
+    rebase(r.a, top_m, c);
+    r.a.s = warp_sum(r.a.s);
+    r.a.v = warp_sum(r.a.v);
+    __syncthreads();  // s.warp's maxima are read
+    if (lane == 0) {
+        s.warp[0][warp] = top_m;
+        s.warp[1][warp] = r.a.s;
+        s.warp[2][warp] = r.a.v;
+    }
+    __syncthreads();
+    if (t == 0) {
+        float m = s.warp[0][0];
+        for (int k = 1; k < kThreads / 32; ++k) m = fmaxf(m, s.warp[0][k]);
+        Stats all{m, 0.0f, 0.0f};
+        for (int k = 0; k < kThreads / 32; ++k) {
+            Stats part{s.warp[0][k], s.warp[1][k], s.warp[2][k]};
+            rebase(part, m, c);
+            all.s += part.s;
+            all.v += part.v;
+        }
+        s.stats = all;
+    }
+    // The share's alternatives.
+    uint32_t count = s.count;
+    if (a.top > 0) {
+        if (count > kCandidates) {
+            select_candidates<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, a.top);
+            count = s.count;
+        }
+        rank_candidates(s, count, a.top);
+    }
+    __syncthreads();
+    if constexpr (kCluster) {
+        // Share 0 joins the others' statistics and alternatives.
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (share == 0) {
+            if (t == 0) {
+                float m = s.stats.m;
+                for (uint32_t k = 1; k < shares; ++k) m = fmaxf(m, cluster.map_shared_rank(&s, k)->stats.m);
+                Stats all = s.stats;
+                rebase(all, m, c);
+                for (uint32_t k = 1; k < shares; ++k) {
+                    Stats part = cluster.map_shared_rank(&s, k)->stats;
+                    rebase(part, m, c);
+                    all.s += part.s;
+                    all.v += part.v;
+                }
+                s.stats = all;
+                s.count = 0;
+            }
+            __syncthreads();
+            for (uint32_t x = t; x < shares * a.top; x += kThreads) {
+                const unsigned long long key = cluster.map_shared_rank(&s, x / a.top)->best[x % a.top];
+                if (key != 0) s.key[atomicAdd(&s.count, 1u)] = key;
+            }
+            __syncthreads();
+            if (a.top > 0) rank_candidates(s, s.count, a.top);
+        }
+        cluster.sync();  // the shares' memory is read
+        if (share != 0) return;
+    }
+    // The list's results.
+    const float m = s.stats.m, sum = s.stats.s;
+    const bool empty = sum == 0.0f;
+    const float log_s = logf(sum);
+    if (t == 0) {
+        if (a.log_sum != nullptr) a.log_sum[i] = empty ? -CUDART_INF_F : m * a.inv_t + log_s;
+        if (a.entropy != nullptr) a.entropy[i] = empty ? 0.0f : log_s - 0.6931471805599453f * s.stats.v / sum;
+    }
+    for (uint32_t g = t; g < a.num_given; g += kThreads) {
+        const uint64_t at = static_cast<uint64_t>(i) * a.num_given + g;
+        if (g >= kThreads) {
+            const int32_t id = a.given[at];
+            given = id >= 0 && static_cast<uint32_t>(id) < n ? to_float(w.z[id]) : -CUDART_INF_F;
+        }
+        a.given_out[at] = given == -CUDART_INF_F ? given : (given - m) * a.inv_t - log_s;
+    }
+    for (uint32_t k = t; k < a.top; k += kThreads) {
+        const uint64_t at = static_cast<uint64_t>(i) * a.top + k;
+        const unsigned long long key = s.best[k];
+        a.top_ids[at] = key == 0 ? -1 : static_cast<int32_t>(index_of(key));
+        a.top_out[at] = key == 0 ? -CUDART_INF_F : (to_float(w.z[index_of(key)]) - m) * a.inv_t - log_s;
+    }
 }
 
-__device__ __forceinline__ float block_sum(float v, float* s) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int w = 0; w < kThreads / 32; ++w) v += s[w];
-    return v;
+template <class T, int kVec, int kThreads, bool kCluster>
+__global__ void __launch_bounds__(kThreads) log_probs_rows_kernel(LogProbsArgs a, uint32_t shares) {
+    __shared__ __align__(16) Shared<kThreads> s;
+    const uint32_t i = kCluster ? blockIdx.x / shares : blockIdx.x;
+    log_probs_list<T, kVec, kThreads, kCluster>(s, a, i, kCluster ? blockIdx.x % shares : 0, kCluster ? shares : 1);
 }
 
-// A CTA per list: the maximum, the sums, then one pass per alternative.
-template <class T>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(LogProbsArgs a) {
-    __shared__ unsigned long long s_key[kThreads / 32];
-    __shared__ float s_sum[kThreads / 32];
+// A list of at most 32 kItems entries by one warp, in registers.
+template <class T, int kItems>
+__device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i, const T* z, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 31;
     const float c = __fmul_rn(kLog2E, a.inv_t);
-    for (uint32_t i = blockIdx.x; i < a.l.lists; i += gridDim.x) {
-        uint64_t first;
-        uint32_t n;
+    float x[kItems];
+    float most = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const uint32_t j = k * 32 + lane;
+        x[k] = j < n ? to_float(z[j]) : -CUDART_INF_F;
+        most = fmaxf(most, x[k]);
+    }
+    float m = warp_max(most);
+    if (m == -CUDART_INF_F) m = -FLT_MAX;
+    float s = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const float y = exponent(x[k], m, c), p = pow2(y);
+        s += p;
+        v = __fmaf_rn(p, y, v);
+    }
+    s = warp_sum(s);
+    v = warp_sum(v);
+    const bool empty = s == 0.0f;
+    const float log_s = logf(s);
+    if (lane == 0) {
+        if (a.log_sum != nullptr) a.log_sum[i] = empty ? -CUDART_INF_F : m * a.inv_t + log_s;
+        if (a.entropy != nullptr) a.entropy[i] = empty ? 0.0f : log_s - 0.6931471805599453f * v / s;
+    }
+    for (uint32_t g = lane; g < a.num_given; g += 32) {
+        const uint64_t at = static_cast<uint64_t>(i) * a.num_given + g;
+        const int32_t id = a.given[at];
+        const float given = id >= 0 && static_cast<uint32_t>(id) < n ? to_float(z[id]) : -CUDART_INF_F;
+        a.given_out[at] = given == -CUDART_INF_F ? given : (given - m) * a.inv_t - log_s;
+    }
+    // The alternatives, one a round: each lane offers its best entry that is not taken (a bit each).
+    uint32_t taken = 0;
+    float out = -CUDART_INF_F;
+    int32_t out_id = -1;
+    uint32_t best = 0, best_k = 0;
+    auto offer = [&] {
+        best = 0;
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const uint32_t o = x[k] == -CUDART_INF_F || ((taken >> k) & 1u) != 0 ? 0u : order_of(x[k]);
+            if (o > best) {
+                best = o;
+                best_k = k;
+            }
+        }
+    };
+    if (a.top > 0) offer();
+    for (uint32_t r = 0; r < a.top; ++r) {
+        const uint32_t most_o = __reduce_max_sync(kFull, best);
+        const uint32_t j = __reduce_min_sync(kFull, best == most_o ? best_k * 32 + lane : 0xFFFFFFFFu);
+        if (most_o != 0 && (r & 31) == lane) out_id = static_cast<int32_t>(j);
+        if (most_o != 0 && (j & 31) == lane) {
+            taken |= 1u << best_k;
+            offer();
+        }
+        if ((r & 31) == 31 || r + 1 == a.top) {  // 32 alternatives leave together
+            const uint32_t base = r & ~31u;
+            if (base + lane < a.top) {
+                const uint64_t at = static_cast<uint64_t>(i) * a.top + base + lane;
+                if (out_id >= 0) out = (to_float(z[out_id]) - m) * a.inv_t - log_s;
+                a.top_ids[at] = out_id;
+                a.top_out[at] = out;
+            }
+            out = -CUDART_INF_F;
+            out_id = -1;
+        }
+    }
+}
+
+// A warp per list; a longer one among them by the whole CTA.
+template <class T>
+__global__ void __launch_bounds__(kWarpThreads) log_probs_warps_kernel(LogProbsArgs a) {
+    __shared__ __align__(16) Shared<kWarpThreads> shared;
+    constexpr uint32_t kLists = kWarpThreads / 32;
+    const uint32_t base = blockIdx.x * kLists, i = base + (threadIdx.x >> 5);
+    uint64_t first = 0;
+    uint32_t n = 0;
+    if (i < a.l.lists) {
         list_range(a.l, i, first, n);
         const T* z = static_cast<const T*>(a.l.scores) + first;
-        unsigned long long best = 0;
-        for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-            const unsigned long long key = order_key(to_float(z[j]), j);
-            best = best > key ? best : key;
-        }
-        best = block_max_key(best, s_key);
-        float m = n > 0 ? to_float(z[0xFFFFFFFFu - static_cast<uint32_t>(best)]) : -CUDART_INF_F;
-        const bool empty = m == -CUDART_INF_F;
-        if (empty) m = 0.0f;
-        float sum = 0.0f, part = 0.0f;
-        for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-            const float d = __fsub_rn(to_float(z[j]), m), e = exp_of(d, c);
-            sum += e;
-            if (e > 0.0f) part += e * d;
-        }
-        sum = block_sum(sum, s_sum);
-        part = block_sum(part, s_sum);
-        const float log_s = logf(sum);
-        if (threadIdx.x == 0) {
-            if (a.log_sum != nullptr) a.log_sum[i] = empty ? -CUDART_INF_F : m * a.inv_t + log_s;
-            if (a.entropy != nullptr) a.entropy[i] = empty ? 0.0f : log_s - part * a.inv_t / sum;
-        }
-        for (uint32_t g = threadIdx.x; g < a.num_given; g += kThreads) {
-            const uint64_t at = static_cast<uint64_t>(i) * a.num_given + g;
-            const int32_t id = a.given[at];
-            a.given_out[at] = id < 0 || static_cast<uint32_t>(id) >= n || empty ? -CUDART_INF_F
-                                                                               : (to_float(z[id]) - m) * a.inv_t - log_s;
-        }
-        unsigned long long last = best;
-        for (uint32_t r = 0; r < a.top; ++r) {
-            if (r > 0) {
-                unsigned long long next = 0;
-                for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-                    const unsigned long long key = order_key(to_float(z[j]), j);
-                    if (key < last && key > next) next = key;
-                }
-                last = block_max_key(next, s_key);
-            }
-            if (threadIdx.x == 0) {
-                const uint64_t at = static_cast<uint64_t>(i) * a.top + r;
-                const uint32_t id = 0xFFFFFFFFu - static_cast<uint32_t>(last);
-                const float v = last == 0 ? -CUDART_INF_F : to_float(z[id]);
-                const bool none = v == -CUDART_INF_F;
-                a.top_ids[at] = none ? -1 : static_cast<int32_t>(id);
-                a.top_out[at] = none ? -CUDART_INF_F : (v - m) * a.inv_t - log_s;
-            }
-        }
+        if (n <= 128)
+            log_probs_warp<T, 4>(a, i, z, n);
+        else if (n <= 256)
+            log_probs_warp<T, 8>(a, i, z, n);
+        else if (n <= kWarpEntries)
+            log_probs_warp<T, 16>(a, i, z, n);
     }
+    if (__syncthreads_or(n > kWarpEntries) == 0) return;
+    for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
+        list_range(a.l, k, first, n);
+        if (n <= kWarpEntries) continue;
+        log_probs_list<T, 1, kWarpThreads, false>(shared, a, k, 0, 1);
+        __syncthreads();
+    }
+}
+
+template <class T, int kVec, int kThreads>
+void launch_rows(const LogProbsArgs& a, uint32_t shares, cudaStream_t s) {
+    if (shares == 1) {
+        log_probs_rows_kernel<T, kVec, kThreads, false><<<a.l.lists, kThreads, 0, s>>>(a, 1);
+        return;
+    }
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.l.lists * shares);
+    config.blockDim = dim3(kThreads);
+    config.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = shares;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, log_probs_rows_kernel<T, kVec, kThreads, true>, a, shares);
+}
+
+template <class T>
+void launch_typed(const LogProbsArgs& a, cudaStream_t s) {
+    constexpr int kVec = 16 / sizeof(T);
+    const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
+    if (mean <= (a.l.bounds != nullptr ? kWarpEntries / 2 : kWarpEntries)) {
+        const uint32_t lists = kWarpThreads / 32;
+        log_probs_warps_kernel<T><<<(a.l.lists + lists - 1) / lists, kWarpThreads, 0, s>>>(a);
+        return;
+    }
+    const uint32_t shares = list_shares(mean, a.l.lists, a.sms);
+    if (a.l.bounds != nullptr)
+        launch_rows<T, 1, 256>(a, shares, s);
+    else if (mean <= 128 * kBatch * kVec)  // one batch of 128 threads holds the list
+        launch_rows<T, kVec, 128>(a, shares, s);
+    else
+        launch_rows<T, kVec, 512>(a, shares, s);
 }
 
 }  // namespace
 
 void launch_log_probs(const LogProbsArgs& a, cudaStream_t s) {
-    const uint32_t most = a.sms * 8, grid = a.l.lists < most ? a.l.lists : most;
     if (a.l.type == SB2_F32)
-        log_probs_kernel<float><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<float>(a, s);
     else if (a.l.type == SB2_BF16)
-        log_probs_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<__nv_bfloat16>(a, s);
     else
-        log_probs_kernel<__half><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<__half>(a, s);
 }
 
 }  // namespace sb2
