@@ -57,6 +57,10 @@ __device__ __forceinline__ uint32_t order_of(float z) {
 __device__ __forceinline__ unsigned long long order_key(float z, uint32_t index) {
     return (static_cast<unsigned long long>(order_of(z)) << 32) | (0xFFFFFFFFu - index);
 }
+// A score from its order (a NaN from a NaN's).
+__device__ __forceinline__ float score_of(uint32_t order) {
+    return __uint_as_float((order >> 31) != 0 ? order & 0x7FFFFFFFu : ~order);
+}
 __device__ __forceinline__ uint32_t index_of(unsigned long long key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
 // 2^x, at most 2 ulp off (ex2.approx); results below 2^-126 are 0.

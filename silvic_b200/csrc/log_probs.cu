@@ -24,6 +24,7 @@ constexpr uint32_t kWarpEntries = 512;
 constexpr int kWarpThreads = 256;        // the warp kernel's CTAs
 constexpr uint32_t kCandidates = 2048;   // keys that a CTA gathers
 constexpr int kBatch = 4;                // vectors a thread holds in flight
+constexpr uint32_t kSingle = 0x80000000u;
 constexpr float kSlack = 4.0f;           // log2 units that an entry may lie above the reference before it moves
 
 struct Stats {
@@ -46,8 +47,9 @@ struct Shared {
     uint32_t order[256];               // group maxima, then the digits' counts
     float warp[3][kThreads / 32];
     Stats stats;
-    float bound;
-    uint32_t count, digit, left;
+    uint32_t bound;                    // the order of the least score of an alternative
+    uint32_t held[kCandidates];        // first entries of vectors that hold candidates (kSingle: an entry alone)
+    uint32_t count, keys, digit, left;
 };
 
 // The share's `top` largest keys of `count` gathered ones into s.best, in order. Few: every key counts the keys above
@@ -60,8 +62,13 @@ __device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t co
     if (count <= 512) {
         for (uint32_t i = t; i < count; i += kThreads) {
             const unsigned long long mine = s.key[i];
-            uint32_t above = 0;
-            for (uint32_t j = 0; j < count; ++j) above += s.key[j] > mine;
+            uint32_t above = 0, j = 0;
+            for (; j + 4 <= count; j += 4) {
+                const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&s.key[j]);
+                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.key[j + 2]);
+                above += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
+            }
+            for (; j < count; ++j) above += s.key[j] > mine;
             if (above < top) s.best[above] = mine;
         }
         return;
@@ -129,52 +136,135 @@ __device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, 
         prefix |= static_cast<unsigned long long>(s.digit) << shift;
         left = s.left;
     }
-    if (threadIdx.x == 0) s.count = 0;
+    if (threadIdx.x == 0) s.keys = 0;
     __syncthreads();
     for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
         const unsigned long long key = order_key(x, j);
         if (x > -CUDART_INF_F && key >= prefix) {
-            const uint32_t at = atomicAdd(&s.count, 1u);
+            const uint32_t at = atomicAdd(&s.keys, 1u);
             if (at < kCandidates) s.key[at] = key;
         }
     });
     __syncthreads();
 }
 
+// The next free slot of a buffer in shared memory. Rarely more than one lane of a warp asks, so the plain atomic is
+// cheaper than one for the warp and a share of it per lane.
+__device__ __forceinline__ uint32_t take(uint32_t* counter) {
+    uint32_t at;
+    asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(counter))) : "memory");
+    return at;
+}
+
+// Statistics about R = m c rounded, so that an exponent is one fma(z, c, -R).
+struct Rounded {
+    Stats a;  // a.m the reference, a.s and a.v about r
+    float r;
+};
+
+// The statistics about m itself: the rounding of R is put back.
+__device__ __forceinline__ Stats settled(const Rounded& x, float c) {
+    if (x.a.s == 0.0f) return {x.a.m, 0.0f, 0.0f};
+    const float y = -__fmaf_rn(x.a.m, c, -x.r), f = pow2(y);
+    return {x.a.m, x.a.s * f, f * __fmaf_rn(x.a.s, y, x.a.v)};
+}
+
+// The statistics about a higher reference.
+__device__ __noinline__ Rounded moved(Rounded x, float m, float c) {
+    Stats now = settled(x, c);
+    rebase(now, m, c);
+    const float r = __fmul_rn(m, c);
+    const float y = __fmaf_rn(m, c, -r), f = pow2(y);
+    return {{m, now.s * f, f * __fmaf_rn(now.s, y, now.v)}, r};
+}
+
 // One thread's running statistics and its filter for alternatives.
 template <class T, int kVec, int kThreads>
 struct Reader {
     Shared<kThreads>& s;
-    Stats a;
+    Rounded x;
     float c, limit, bound;
 
-    __device__ __forceinline__ void gather(float x, uint32_t j) {
-        if (x >= bound && x > -CUDART_INF_F) {
-            const uint32_t at = atomicAdd(&s.count, 1u);
-            if (at < kCandidates) s.key[at] = order_key(x, j);
-        }
+    // About the maximum of the first entries (-inf: about the first unmasked entry that comes).
+    __device__ __forceinline__ Reader(Shared<kThreads>& shared, float m, float scale, float bound_)
+        : s(shared), c(scale), limit(m + kSlack / scale), bound(bound_) {
+        x.a = {fmaxf(m, -FLT_MAX), 0.0f, 0.0f};
+        x.r = m == -CUDART_INF_F ? 0.0f : __fmul_rn(m, scale);
     }
+    // Whether R is so large that its rounding matters: far_stats() takes over.
+    __device__ __forceinline__ bool far() const { return !(fabsf(x.r) < 1048576.0f); }
     template <int kCount>
-    __device__ __forceinline__ void add(const float (&x)[kCount], uint32_t first) {
-        float most = x[0];
+    __device__ __forceinline__ void add(const float (&z)[kCount], uint32_t first) {
+        float most = z[0];
 #pragma unroll
-        for (int e = 1; e < kCount; ++e) most = fmaxf(most, x[e]);
+        for (int e = 1; e < kCount; ++e) most = fmaxf(most, z[e]);
         if (most > limit) {
-            rebase(a, most, c);
+            x = moved(x, most, c);
             limit = most + kSlack / c;
         }
+        if constexpr (kCount == 1) {
+            const float y = max_nan(__fmaf_rn(z[0], c, -x.r), -200.0f), p = pow2(y);
+            x.a.s += p;
+            x.a.v = __fmaf_rn(p, y, x.a.v);
+        } else {
+            // pairs in one instruction: issue bounds the kernel before memory
+            const float2 cc = make_float2(c, c), minus_r = make_float2(-x.r, -x.r);
+            float2 sum = make_float2(0.0f, 0.0f), part = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < kCount; ++e) {
-            const float y = exponent(x[e], a.m, c), p = pow2(y);
-            a.s += p;
-            a.v = __fmaf_rn(p, y, a.v);
+            for (int e = 0; e < kCount; e += 2) {
+                float2 y = __ffma2_rn(make_float2(z[e], z[e + 1]), cc, minus_r);
+                y.x = max_nan(y.x, -200.0f);  // a masked entry's 0 times its exponent is 0
+                y.y = max_nan(y.y, -200.0f);
+                const float2 p = make_float2(pow2(y.x), pow2(y.y));
+                sum = __fadd2_rn(sum, p);
+                part = __ffma2_rn(p, y, part);
+            }
+            x.a.s += sum.x + sum.y;
+            x.a.v += part.x + part.y;
         }
-        if (most >= bound && s.count <= kCandidates) {
-#pragma unroll
-            for (int e = 0; e < kCount; ++e) gather(x[e], first + e);
+        if (most >= bound) {  // the vector (or the scalar) holds a candidate
+            const uint32_t at = take(&s.count);
+            if (at < kCandidates) s.held[at] = kCount == 1 ? first | kSingle : first;
         }
     }
 };
+
+// The statistics of a share of far scores (about 700,000 T and more from 0): the maximum first, then each entry's distance from it.
+template <class T, int kVec, int kThreads>
+__device__ __noinline__ Stats far_stats(Shared<kThreads>& s, const T* z, uint32_t n, uint32_t from, uint32_t to, bool edges,
+                                        float c) {
+    const Walk<T, kVec> w(z, n);
+    Stats a{-FLT_MAX, 0.0f, 0.0f};
+    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t) { a.m = fmaxf(a.m, x); });
+    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t) {
+        const float y = exponent(x, a.m, c), p = pow2(y);
+        a.s += p;
+        a.v = __fmaf_rn(p, y, a.v);
+    });
+    return a;
+}
+
+// The candidates' keys: entries of the held vectors that reach the bound. False: more than the buffer holds.
+template <class T, int kVec, int kThreads>
+__device__ __forceinline__ bool expand(Shared<kThreads>& s, const T* z, float bound) {
+    __syncthreads();
+    const uint32_t count = s.count;
+    if (count > kCandidates) return false;
+    if (threadIdx.x == 0) s.keys = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count * kVec; i += kThreads) {
+        const uint32_t held = s.held[i / kVec], e = i % kVec;
+        const uint32_t j = (held & ~kSingle) + e;
+        if ((held & kSingle) != 0 && e > 0) continue;
+        const float x = to_float(z[j]);
+        if (x >= bound) {
+            const uint32_t at = take(&s.keys);
+            if (at < kCandidates) s.key[at] = order_key(x, j);
+        }
+    }
+    __syncthreads();
+    return s.keys <= kCandidates;
+}
 
 // One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1).
 template <class T, int kVec, int kThreads, bool kCluster>
@@ -224,79 +314,83 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     if (lane == 0) s.warp[0][warp] = most;
     if (t == 0) {
         s.count = 0;
-        s.bound = -CUDART_INF_F;
+        s.bound = 0xFFFFFFFFu;
     }
     __syncthreads();
     most = s.warp[0][0];
 #pragma unroll
     for (int k = 1; k < kThreads / 32; ++k) most = fmaxf(most, s.warp[0][k]);
-    if (a.top == 0) {
-        if (t == 0) s.bound = CUDART_INF_F;
-    } else if (t < groups) {
+    if (a.top > 0 && t < groups) {  // the least group that fewer than `top` others exceed
         const uint32_t mine = s.order[t];
         uint32_t above = 0;
         for (uint32_t j = 0; j < groups; j += 4) {
             const uint4 o = *reinterpret_cast<const uint4*>(&s.order[j]);
-            above += (o.x > mine || (o.x == mine && j < t)) + (o.y > mine || (o.y == mine && j + 1 < t)) +
-                     (o.z > mine || (o.z == mine && j + 2 < t)) + (o.w > mine || (o.w == mine && j + 3 < t));
+            above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
         }
-        if (above == a.top - 1) s.bound = __uint_as_float((mine >> 31) != 0 ? mine & 0x7FFFFFFFu : ~mine);
+        const uint32_t least = __reduce_min_sync(kFull, above < a.top ? mine : 0xFFFFFFFFu);
+        if (lane == 0) atomicMin(&s.bound, least);
     }
     __syncthreads();
+    // Masked entries are no alternatives.
+    const float bound = a.top > 0 ? fmaxf(score_of(s.bound), -FLT_MAX) : CUDART_NAN_F;
     // One pass: the statistics about the first batch's maximum (moved where later entries lie far above it), and the
     // entries that reach the bound.
-    Reader<T, kVec, kThreads> r{s, {most == -CUDART_INF_F ? -FLT_MAX : most, 0.0f, 0.0f}, c, 0.0f, s.bound};
-    r.limit = r.a.m + kSlack / c;
-    for (uint32_t v = from + t; v < to; v += kBatch * kThreads) {
-        Pack<T, kVec> now[kBatch];
+    Reader<T, kVec, kThreads> r(s, most, c, bound);
+    uint32_t batch = 0;
+    for (uint32_t base = from; base < to; base += kBatch * kThreads) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            now[u] = p[u];
-            const uint32_t next = v + (u + kBatch) * kThreads;
-            if (next < to) p[u].load(w.z + w.at(next));
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            if (v + u * kThreads < to) {
+            const uint32_t v = base + u * kThreads + t;
+            if (v < to) {
                 float x[kVec];
-                now[u].values(x);
-                r.add(x, w.at(v + u * kThreads));
+                p[u].values(x);
+                const uint32_t next = v + kBatch * kThreads;
+                if (next < to) p[u].load(w.z + w.at(next));
+                r.add(x, w.at(v));
             }
+        }
+        // Each time the part that is read has doubled: many candidates are cut to the alternatives so far, whose last
+        // is the bound from here on. So candidates stay few however long the list is, unless its order defeats that.
+        if ((++batch & (batch - 1)) == 0 && a.top > 0 && base + kBatch * kThreads < to) {
+            __syncthreads();
+            if (s.count > max(64u, 2 * a.top) && expand<T, kVec, kThreads>(s, w.z, r.bound)) {
+                rank_candidates(s, s.keys, a.top);
+                __syncthreads();
+                for (uint32_t k = t; k < a.top; k += kThreads) s.held[k] = index_of(s.best[k]) | kSingle;
+                r.bound = score_of(static_cast<uint32_t>(s.best[a.top - 1] >> 32));
+                if (t == 0) s.count = a.top;
+            }
+            __syncthreads();
         }
     }
     if (edge_at < n) r.add(edge, edge_at);
     // The share's statistics.
-    const float top_m = warp_max(r.a.m);
-    rebase(r.a, top_m, c);
-    r.a.s = warp_sum(r.a.s);
-    r.a.v = warp_sum(r.a.v);
-    __syncthreads();  // s.warp's maxima are read
+    Stats mine = settled(r.x, c);
+    if (__syncthreads_or(r.far())) mine = far_stats<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, c);
+    const float top_m = warp_max(mine.m);
+    rebase(mine, top_m, c);
+    mine.s = warp_sum(mine.s);
+    mine.v = warp_sum(mine.v);
     if (lane == 0) {
         s.warp[0][warp] = top_m;
-        s.warp[1][warp] = r.a.s;
-        s.warp[2][warp] = r.a.v;
+        s.warp[1][warp] = mine.s;
+        s.warp[2][warp] = mine.v;
     }
     __syncthreads();
-    if (t == 0) {
-        float m = s.warp[0][0];
-        for (int k = 1; k < kThreads / 32; ++k) m = fmaxf(m, s.warp[0][k]);
-        Stats all{m, 0.0f, 0.0f};
-        for (int k = 0; k < kThreads / 32; ++k) {
-            Stats part{s.warp[0][k], s.warp[1][k], s.warp[2][k]};
-            rebase(part, m, c);
-            all.s += part.s;
-            all.v += part.v;
-        }
-        s.stats = all;
+    if (warp == 0) {
+        Stats part{-FLT_MAX, 0.0f, 0.0f};
+        if (lane < kThreads / 32) part = {s.warp[0][lane], s.warp[1][lane], s.warp[2][lane]};
+        const float m = warp_max(part.m);
+        rebase(part, m, c);
+        part.s = warp_sum(part.s);
+        part.v = warp_sum(part.v);
+        if (lane == 0) s.stats = {m, part.s, part.v};
     }
     // The share's alternatives.
-    uint32_t count = s.count;
     if (a.top > 0) {
-        if (count > kCandidates) {
+        if (!expand<T, kVec, kThreads>(s, w.z, r.bound))
             select_candidates<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, a.top);
-            count = s.count;
-        }
-        rank_candidates(s, count, a.top);
+        rank_candidates(s, s.keys, a.top);
     }
     __syncthreads();
     if constexpr (kCluster) {
@@ -316,15 +410,15 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
                     all.v += part.v;
                 }
                 s.stats = all;
-                s.count = 0;
+                s.keys = 0;
             }
             __syncthreads();
             for (uint32_t x = t; x < shares * a.top; x += kThreads) {
                 const unsigned long long key = cluster.map_shared_rank(&s, x / a.top)->best[x % a.top];
-                if (key != 0) s.key[atomicAdd(&s.count, 1u)] = key;
+                if (key != 0) s.key[atomicAdd(&s.keys, 1u)] = key;
             }
             __syncthreads();
-            if (a.top > 0) rank_candidates(s, s.count, a.top);
+            if (a.top > 0) rank_candidates(s, s.keys, a.top);
         }
         cluster.sync();  // the shares' memory is read
         if (share != 0) return;
@@ -495,7 +589,9 @@ void launch_typed(const LogProbsArgs& a, cudaStream_t s) {
         launch_rows<T, 1, 256>(a, shares, s);
     else if (mean <= 128 * kBatch * kVec)  // one batch of 128 threads holds the list
         launch_rows<T, kVec, 128>(a, shares, s);
-    else
+    else if (shares == 1)  // small CTAs: one's barriers hide behind the others' reading
+        launch_rows<T, kVec, 256>(a, 1, s);
+    else  // SMs to spare: more threads a list
         launch_rows<T, kVec, 512>(a, shares, s);
 }
 

@@ -582,3 +582,27 @@ def test_objective_refuses_bad_queries_and_teachers(device):
         b.load(data, "distill")  # a new dataset asks for its teacher again
         with pytest.raises(SilvicError, match="no teacher"):
             b.compute_gradients()
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("lists,width", [(3, 5000), (300, 20011)])
+def test_log_probs_of_far_scores(backend, type_, lists, width):
+    """Scores so far from 0 that m log2(e) / T rounds by whole units, or passes f32; first entries all masked; a list
+    that climbs far above its first entries."""
+    rng = np.random.RandomState(width)
+    z = rng.randn(lists, width) * 3
+    z[0] = -1.0e30
+    z[0, ::7] *= 1.0 + 2.0 ** -7
+    z[1] += 4.0e6
+    z[2, : width - 50] = -np.inf
+    if lists > 3:
+        z[3] += np.linspace(-300, 300, width)
+        z[4, : width - 40] = -np.inf
+        z[4, width - 40:] = torch.finfo(TYPES[type_]).min
+        z[5, : width - 40] = -1.0e5
+    scores = torch.from_numpy(z).to(TYPES[type_]).cuda()
+    ids = np.stack([np.arange(lists) % width, np.full(lists, width - 1)], 1).astype(np.int32)
+    for t in (1.0, 0.01):
+        got = backend.log_probs(scores, given=torch.from_numpy(ids).cuda(), top=9, temperature=t)
+        check_log_probs(scores[:12], rows_of(scores[:12]), ids, 9, t,
+                        type(got)(*[v[:12] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
