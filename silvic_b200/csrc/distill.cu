@@ -8,151 +8,651 @@
 //            w / T p_j (Q - r / P)          elsewhere
 //   hess_j = w / T^2 Q p_j (1 - p_j)        (the diagonal of the softmax's own second derivative)
 // P is summed over the entries outside the top, not taken as 1 - sum p: a student that has learned its teacher keeps
-// little there.
+// little there. The top's entries are marked in a bitmap, which the sum skips; their gradients are written once the
+// others are, over what the common formula left there. An entry named twice has its q added in the teacher's order.
+//
+// Lists of at most kWarpEntries take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
+// holds it in registers between the sums and the gradients, so that memory sees each score once. A list too long for
+// that (or of scores so far from 0 that fma(z, c, -m c) loses its last bits) is read again for each pass.
+#include <cfloat>
+
 #include "lists_device.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace sb2 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr uint32_t kWarpEntries = 512;
+constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
+constexpr float kFar = 1048576.0f;   // |m c| from which an exponent is taken from the distance z - m
 
-__device__ __forceinline__ float block_sum(float v, float* s) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int w = 0; w < kThreads / 32; ++w) v += s[w];
+// What a CTA keeps of its share of a list; kBits entries have a bit of their own, more share them.
+template <int kThreads, int kBits>
+struct Shared {
+    float warp[7][kThreads / 32];
+    float m, outside;                // the share's reference, and its sum (outside the top, where the rest counts)
+    int32_t id[kMaxTop];
+    float q[kMaxTop];
+    uint32_t edge_bits;              // marks of the scalars outside the vectors
+    uint32_t bits[kBits / 32];
+};
+
+template <int kThreads>
+__device__ __forceinline__ float sum_of(const float (&part)[kThreads / 32]) {
+    float v = part[0];
+#pragma unroll
+    for (int k = 1; k < kThreads / 32; ++k) v += part[k];
     return v;
 }
 
-__device__ __forceinline__ float block_max(float v, float* s) {
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = s[0];
-    for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, s[w]);
+template <int kThreads>
+__device__ __forceinline__ float max_of(const float (&part)[kThreads / 32]) {
+    float v = part[0];
+#pragma unroll
+    for (int k = 1; k < kThreads / 32; ++k) v = fmaxf(v, part[k]);
     return v;
 }
 
-// A CTA per list: the teacher's q, the maximum, the sums in and outside the top, then the gradients.
+// What the derivatives of a list's entries share: with e = exp((z - m) / T) and p = inv_s e, the gradient is slope e
+// outside the top and top_slope e less q in it, the hessian curve p (1 - p).
+struct Slopes {
+    float inv_s, slope, top_slope, curve;
+};
+
+// Writes an entry's derivatives; the objective's row weight and maxima come in here.
+struct Maxima {
+    float g = 0.0f, h = 0.0f;
+};
 template <class T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a) {
+__device__ __forceinline__ void put(const DistillArgs& a, uint64_t to, uint64_t row, float g, float h, bool counts, Maxima& most) {
+    if (a.row_weight != nullptr) {
+        g *= a.row_weight[row];
+        h *= a.row_weight[row];
+    }
+    if (counts) {
+        most.g = fmaxf(most.g, fabsf(g));
+        most.h = fmaxf(most.h, fabsf(h));
+    }
+    if (a.grad != nullptr) static_cast<T*>(a.grad)[to] = from_float<T>(g);
+    if (a.hess != nullptr) static_cast<T*>(a.hess)[to] = from_float<T>(h);
+}
+
+// A CTA's maxima over its lists, for a training iteration.
+template <int kThreads>
+__device__ __forceinline__ void publish(const DistillArgs& a, Maxima most) {
+    if (a.max_g == nullptr) return;
+    __shared__ float s_g[kThreads / 32], s_h[kThreads / 32];
+    most.g = warp_max(most.g);
+    most.h = warp_max(most.h);
+    if ((threadIdx.x & 31) == 0) {
+        s_g[threadIdx.x >> 5] = most.g;
+        s_h[threadIdx.x >> 5] = most.h;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {  // non-negative doubles order like their bit patterns
+        atomicMax(a.max_g, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(max_of<kThreads>(s_g)))));
+        atomicMax(a.max_h, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(max_of<kThreads>(s_h)))));
+    }
+}
+
+// Eight (four) derivatives as one 16-byte vector.
+template <class T, int kVec>
+__device__ __forceinline__ uint4 packed(const float (&v)[kVec]) {
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+            } else {
+                const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// One entry of the teacher's top: its index (-1: padding), t / T and the student's score there.
+__device__ __forceinline__ void teacher_entry(const DistillArgs& a, uint32_t i, uint32_t k, uint32_t n, int32_t& id, float& y) {
+    const uint64_t at = static_cast<uint64_t>(i) * a.t.stride + k;
+    id = a.t.ids[at];
+    if (id < 0 || static_cast<uint32_t>(id) >= n) id = -1;
+    y = id >= 0 ? load_typed(a.t.logits, a.t.type, at) * a.inv_t : -CUDART_INF_F;
+}
+
+// The loss of a list from its parts: sum q (log q - (z - m) / T), sum q, the sums S and S P, and the rest.
+__device__ __forceinline__ float loss_of(float cross, float held, float sum, float outside, float r) {
+    const float log_s = logf(sum);
+    float loss = cross + held * log_s;
+    if (r > 0.0f) loss += r * (logf(r) - (logf(outside) - log_s));
+    return loss;
+}
+
+__device__ __forceinline__ Slopes slopes_of(float w, float inv_t, float held, float r, float sum, float outside) {
+    Slopes k;
+    const float mass = held + r;
+    k.inv_s = 1.0f / sum;
+    k.top_slope = mass * k.inv_s * (w * inv_t);
+    k.slope = r > 0.0f ? (mass * k.inv_s - r / outside) * (w * inv_t) : k.top_slope;
+    k.curve = mass * (w * inv_t * inv_t);
+    return k;
+}
+
+// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). kHeld vectors a thread
+// stay in registers.
+template <class T, int kVec, int kHeld, int kThreads, bool kCluster>
+__device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kThreads>& s, const DistillArgs& a, uint32_t i,
+                                             uint32_t share, uint32_t shares, Maxima& most) {
+    constexpr uint32_t kBits = kVec * kHeld * kThreads;
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    uint64_t first;
+    uint32_t n;
+    list_range(a.l, i, first, n);
+    const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
+    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * share / shares);
+    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * (share + 1) / shares);
+    const float c = __fmul_rn(kLog2E, a.inv_t);
+    const bool rest = a.t.log_sum != nullptr, marks = rest || a.max_g != nullptr;
+    const bool held_here = to - from <= kHeld * kThreads;
+    // The scores, on their way.
+    Pack<T, kVec> p[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        const uint32_t v = from + u * kThreads + t;
+        if (held_here && v < to)
+            p[u].load(w.z + w.at(v));
+        else
+            p[u].masked();
+    }
+    const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
+    const float edge = edge_at < n ? to_float(w.z[edge_at]) : -CUDART_INF_F;
+    // The teacher, and the marks of its entries in this share.
+    int32_t id = -1;
+    float y = -CUDART_INF_F, zt = -CUDART_INF_F;
+    if (t < a.t.top) {
+        teacher_entry(a, i, t, n, id, y);
+        if (id >= 0) zt = to_float(w.z[id]);
+        s.id[t] = id;
+    }
+    if (marks) {
+        const uint32_t words = min(kBits, (to - from) * kVec + 31) / 32;
+        for (uint32_t k = t; k < words; k += kThreads) s.bits[k] = 0;
+        if (t == 0) s.edge_bits = 0;
+        __syncthreads();
+        if (id >= 0) {
+            const uint32_t j = static_cast<uint32_t>(id);
+            if (j < w.head || j >= w.tail()) {
+                atomicOr(&s.edge_bits, 1u << (j < w.head ? j : w.head + (j - w.tail())));
+            } else if ((j - w.head) / kVec >= from && (j - w.head) / kVec < to) {
+                const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
+                atomicOr(&s.bits[bit / 32], 1u << (bit & 31));
+            }
+        }
+    }
+    // Marks of vector `v`'s entries. Entries that share bits (a list too long for the registers) look among the ids.
+    auto marked = [&](uint32_t v) {
+        const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
+        uint32_t m = (s.bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
+        if (!held_here && m != 0) {
+            m = 0;
+            for (uint32_t k = 0; k < a.t.top; ++k) {
+                const uint32_t e = static_cast<uint32_t>(s.id[k]) - w.at(v);
+                if (e < kVec) m |= 1u << e;
+            }
+        }
+        return m;
+    };
+    // The maxima of the scores and of the teacher's.
+    float m = fmaxf(edge, zt);  // with the top's scores, so that no share's reference lies far below them
+    if (held_here) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            float x[kVec];
+            p[u].values(x);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) m = fmaxf(m, x[e]);
+        }
+    } else {
+        for (uint32_t v = from + t; v < to; v += kThreads) {
+            Pack<T, kVec> now;
+            float x[kVec];
+            now.load(w.z + w.at(v));
+            now.values(x);
+            for (int e = 0; e < kVec; ++e) m = fmaxf(m, x[e]);
+        }
+    }
+    m = warp_max(m);
+    float y_max = warp_max(y);
+    if (lane == 0) {
+        s.warp[0][warp] = m;
+        s.warp[1][warp] = y_max;
+    }
+    const bool taught = __syncthreads_or(id >= 0) != 0;
+    m = fmaxf(max_of<kThreads>(s.warp[0]), -FLT_MAX);
+    y_max = fmaxf(max_of<kThreads>(s.warp[1]), -FLT_MAX);
+    float R = __fmul_rn(m, c);
+    bool far = !(fabsf(R) < kFar) || !held_here;
+    // The share's sum (with the rest, outside the top), the top's own and the teacher's.
+    float sum = 0.0f;
+    if (!far) {
+        const float2 cc = make_float2(c, c), minus_r = make_float2(-R, -R);
+        float2 two = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            const uint32_t v = from + u * kThreads + t;
+            if (v >= to) break;
+            float x[kVec];
+            p[u].values(x);
+            if constexpr (kVec == 1) {
+                const float e = pow2(__fmaf_rn(x[0], c, -R));
+                if (!rest || marked(v) == 0) sum += e;
+            } else {
+                const uint32_t skip = rest ? marked(v) : 0;
+                if (skip != 0) {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        if ((skip >> e) & 1u) x[e] = -CUDART_INF_F;
+                }
+#pragma unroll
+                for (int e = 0; e < kVec; e += 2) {
+                    const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), cc, minus_r);
+                    two = __fadd2_rn(two, make_float2(pow2(z.x), pow2(z.y)));
+                }
+            }
+        }
+        sum += two.x + two.y;
+    } else {
+        for (uint32_t v = from + t; v < to; v += kThreads) {
+            Pack<T, kVec> now;
+            float x[kVec];
+            now.load(w.z + w.at(v));
+            now.values(x);
+            const uint32_t skip = rest ? marked(v) : 0;
+            for (int e = 0; e < kVec; ++e)
+                if (((skip >> e) & 1u) == 0) sum += pow2(exponent(x[e], m, c));
+        }
+    }
+    auto term = [&](float z) { return far ? pow2(exponent(z, m, c)) : pow2(__fmaf_rn(z, c, -R)); };
+    const bool edge_marked = marks && edge_at < n && ((s.edge_bits >> t) & 1u) != 0;
+    if (edge_at < n && !(rest && edge_marked)) sum += term(edge);
+    bool leads = id >= 0, alone = true;
+    if (t < a.t.top) {
+        for (uint32_t k = 0; k < a.t.top; ++k)
+            if (s.id[k] == id && k != t) {
+                alone = false;
+                if (k < t) leads = false;
+            }
+    }
+    const float e_t = id >= 0 ? term(zt) : 0.0f;
+    float top_sum = rest && leads ? e_t : 0.0f;
+    float total = rest || id < 0 ? 0.0f : expf(y - y_max);
+    sum = warp_sum(sum);
+    top_sum = warp_sum(top_sum);
+    total = warp_sum(total);
+    if (lane == 0) {
+        s.warp[2][warp] = sum;
+        s.warp[3][warp] = top_sum;
+        s.warp[4][warp] = total;
+    }
+    __syncthreads();
+    // About m itself: the rounding of R is put back.
+    const float settle = far ? 1.0f : pow2(-__fmaf_rn(m, c, -R));
+    float outside = settle * sum_of<kThreads>(s.warp[2]);
+    top_sum = settle * sum_of<kThreads>(s.warp[3]);
+    total = sum_of<kThreads>(s.warp[4]);
+    if constexpr (kCluster) {
+        // Every share's sum is about its own reference: their sum is about the largest.
+        cg::cluster_group cluster = cg::this_cluster();
+        if (t == 0) {
+            s.m = m;
+            s.outside = outside;
+        }
+        cluster.sync();
+        float all = -FLT_MAX;
+        for (uint32_t k = 0; k < shares; ++k) all = fmaxf(all, cluster.map_shared_rank(&s, k)->m);
+        float joined = 0.0f;
+        for (uint32_t k = 0; k < shares; ++k) {
+            const auto* other = cluster.map_shared_rank(&s, k);
+            joined += other->outside * pow2(exponent(other->m, all, c));
+        }
+        outside = joined;
+        top_sum *= pow2(exponent(m, all, c));
+        m = all;
+        R = __fmul_rn(m, c);
+        far = !(fabsf(R) < kFar) || !held_here;
+        cluster.sync();  // the shares' memory is read
+    }
+    sum = outside + top_sum;
+    // The teacher's q, and the loss.
+    float log_q = -CUDART_INF_F;
+    if (id >= 0) log_q = rest ? y - a.t.log_sum[i] : total == 0.0f ? -CUDART_INF_F : y - y_max - logf(total);
+    const float q = expf(log_q);
+    if (t < a.t.top) s.q[t] = q;
+    float held = warp_sum(q);
+    float cross = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
+    if (lane == 0) {
+        s.warp[5][warp] = held;
+        s.warp[6][warp] = cross;
+    }
+    __syncthreads();
+    held = sum_of<kThreads>(s.warp[5]);
+    cross = sum_of<kThreads>(s.warp[6]);
+    const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+    const bool empty = sum == 0.0f || !taught;
+    const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
+    if (t == 0 && share == 0 && a.loss != nullptr) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+    if (a.grad == nullptr && a.hess == nullptr) return;
+    // The derivatives outside the top, and what the same formula gives in it.
+    Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
+    if (!far) {  // the terms are about R
+        const float f = pow2(-__fmaf_rn(m, c, -R));
+        k.inv_s *= f;
+        k.slope *= f;
+        k.top_slope *= f;
+    }
+    const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
+    auto put_one = [&](float z, uint32_t j, bool counts) {
+        const float e = empty ? 0.0f : term(z), q_j = e * k.inv_s;
+        put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * e, empty ? 0.0f : k.curve * q_j * (1.0f - q_j), counts, most);
+    };
+    if (!far && !empty) {
+        T* const grad = a.grad != nullptr ? static_cast<T*>(a.grad) + out : nullptr;
+        T* const hess = a.hess != nullptr ? static_cast<T*>(a.hess) + out : nullptr;
+        const bool aligned = kVec > 1 && ((reinterpret_cast<uintptr_t>(grad + w.head) | reinterpret_cast<uintptr_t>(hess + w.head)) & 15) == 0;
+        const float2 cc = make_float2(c, c), minus_r = make_float2(-R, -R), slope = make_float2(k.slope, k.slope);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            const uint32_t v = from + u * kThreads + t;
+            if (v >= to) break;
+            float x[kVec];
+            p[u].values(x);
+            if constexpr (kVec == 1) {
+                put_one(x[0], w.at(v), a.max_g == nullptr || marked(v) == 0);
+            } else {
+                float g[kVec], h[kVec];
+#pragma unroll
+                for (int e = 0; e < kVec; e += 2) {
+                    const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), cc, minus_r);
+                    const float2 two = __fmul2_rn(make_float2(x[e] = pow2(z.x), x[e + 1] = pow2(z.y)), slope);
+                    g[e] = two.x;
+                    g[e + 1] = two.y;
+                }
+                if (hess != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        const float q_j = x[e] * k.inv_s;
+                        h[e] = k.curve * q_j * (1.0f - q_j);
+                    }
+                }
+                const uint32_t j = w.at(v);
+                if (aligned) {
+                    if (grad != nullptr) __stcs(reinterpret_cast<uint4*>(grad + j), packed<T, kVec>(g));
+                    if (hess != nullptr) __stcs(reinterpret_cast<uint4*>(hess + j), packed<T, kVec>(h));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        if (grad != nullptr) grad[j + e] = from_float<T>(g[e]);
+                        if (hess != nullptr) hess[j + e] = from_float<T>(h[e]);
+                    }
+                }
+            }
+        }
+    } else {
+        for (uint32_t v = from + t; v < to; v += kThreads) {
+            const uint32_t skip = a.max_g != nullptr ? marked(v) : 0;
+            for (int e = 0; e < kVec; ++e) put_one(to_float(w.z[w.at(v) + e]), w.at(v) + e, ((skip >> e) & 1u) == 0);
+        }
+    }
+    if (edge_at < n) put_one(edge, edge_at, !edge_marked);
+    __syncthreads();
+    // The top's own, over them.
+    if (leads && !empty) {
+        const uint32_t j = static_cast<uint32_t>(id);
+        const bool scalar = j < w.head || j >= w.tail();
+        const uint32_t v = scalar ? 0 : (j - w.head) / kVec;
+        if (scalar ? share == 0 : v >= from && v < to) {
+            float taught_q = q;
+            if (!alone) {
+                taught_q = 0.0f;
+                for (uint32_t x = 0; x < a.t.top; ++x)
+                    if (s.id[x] == id) taught_q += s.q[x];
+            }
+            const float e = term(zt), p_j = e * k.inv_s;
+            put<T>(a, out + j, first + j, k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p_j * (1.0f - p_j), true, most);
+        }
+    }
+}
+
+template <class T, int kVec, int kHeld, int kThreads, bool kCluster>
+__global__ void __launch_bounds__(kThreads, kVec == 1 ? 1 : 1024 / kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares) {
     if (a.stopped != nullptr && *a.stopped) return;
-    __shared__ float s_red[kThreads / 32];
-    __shared__ int32_t s_id[kMaxTop];
-    __shared__ float s_q[kMaxTop];
+    __shared__ Shared<kThreads, kVec * kHeld * kThreads> s;
+    Maxima most;
+    const uint32_t i = kCluster ? blockIdx.x / shares : blockIdx.x;
+    distill_list<T, kVec, kHeld, kThreads, kCluster>(s, a, i, kCluster ? blockIdx.x % shares : 0, kCluster ? shares : 1, most);
+    publish<kThreads>(a, most);
+}
+
+// A warp's teacher: its marks (a bit an entry of the list), ids and q.
+struct WarpShared {
+    uint32_t bits[kWarpEntries / 32];
+    int32_t id[kMaxTop];
+    float q[kMaxTop];
+};
+
+// A list of at most 32 kItems entries by one warp, in registers; kTop of the teacher's entries a lane.
+template <class T, int kItems, int kTop>
+__device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n, Maxima& most) {
+    const uint32_t lane = threadIdx.x & 31;
+    const T* z = static_cast<const T*>(a.l.scores) + first;
     const float c = __fmul_rn(kLog2E, a.inv_t);
     const bool rest = a.t.log_sum != nullptr;
-    const uint32_t k = a.t.top;
-    float most_g = 0.0f, most_h = 0.0f;
-    for (uint32_t i = blockIdx.x; i < a.l.lists; i += gridDim.x) {
-        uint64_t first;
-        uint32_t n;
-        list_range(a.l, i, first, n);
-        const T* z = static_cast<const T*>(a.l.scores) + first;
-        // The teacher: entry threadIdx.x of the top (kMaxTop <= kThreads).
-        int32_t id = -1;
-        float y = -CUDART_INF_F;
-        if (threadIdx.x < k) {
-            id = a.t.ids[static_cast<uint64_t>(i) * a.t.stride + threadIdx.x];
-            if (id < 0 || static_cast<uint32_t>(id) >= n) id = -1;
-            if (id >= 0) y = load_typed(a.t.logits, a.t.type, static_cast<uint64_t>(i) * a.t.stride + threadIdx.x) * a.inv_t;
+    float x[kItems], m = -CUDART_INF_F;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        const uint32_t j = u * 32 + lane;
+        x[u] = j < n ? to_float(z[j]) : -CUDART_INF_F;
+        m = fmaxf(m, x[u]);
+    }
+    int32_t id[kTop];
+    float y[kTop], zt[kTop], y_max = -CUDART_INF_F;
+    bool taught = false;
+    if (lane < kItems) s.bits[lane] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kTop; ++u) {
+        id[u] = -1;
+        y[u] = zt[u] = -CUDART_INF_F;
+        const uint32_t k = u * 32 + lane;
+        if (k < a.t.top) {
+            teacher_entry(a, i, k, n, id[u], y[u]);
+            s.id[k] = id[u];
         }
-        float log_q;
-        if (rest) {
-            log_q = y - a.t.log_sum[i];
-            if (id < 0) log_q = -CUDART_INF_F;
+        if (id[u] >= 0) {
+            zt[u] = to_float(z[id[u]]);
+            atomicOr(&s.bits[id[u] / 32], 1u << (id[u] & 31));
+            taught = true;
+        }
+        y_max = fmaxf(y_max, y[u]);
+    }
+    m = fmaxf(warp_max(m), -FLT_MAX);
+    y_max = fmaxf(warp_max(y_max), -FLT_MAX);
+    taught = __any_sync(kFull, taught);  // and the marks are set
+    uint32_t marks = 0;
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        const bool mark = ((s.bits[u] >> lane) & 1u) != 0;
+        marks |= mark ? 1u << u : 0u;
+        x[u] = pow2(exponent(x[u], m, c));
+        if (!(rest && mark)) sum += x[u];
+    }
+    // Leaders: the first entry of the teacher that names an index.
+    float top_sum = 0.0f, total = 0.0f;
+    uint32_t leads = 0, alone = 0;
+#pragma unroll
+    for (int u = 0; u < kTop; ++u) {
+        bool first_one = id[u] >= 0, only = true;
+        if (kTop == 1) {
+            const uint32_t same = __match_any_sync(kFull, id[u]);
+            first_one = first_one && static_cast<uint32_t>(__ffs(same) - 1) == lane;
+            only = same == 1u << lane;
         } else {
-            float most = block_max(y, s_red);
-            if (most == -CUDART_INF_F) most = 0.0f;
-            const float total = block_sum(expf(y - most), s_red);
-            log_q = total == 0.0f ? -CUDART_INF_F : y - most - logf(total);
-        }
-        const float q = expf(log_q);
-        const bool taught_at_all = __syncthreads_or(id >= 0) != 0;
-        float held = block_sum(q, s_red);
-        __syncthreads();
-        if (threadIdx.x < k) {
-            s_id[threadIdx.x] = id;
-            s_q[threadIdx.x] = q;
-        }
-        __syncthreads();
-        // The student.
-        float m = -CUDART_INF_F;
-        for (uint32_t j = threadIdx.x; j < n; j += kThreads) m = fmaxf(m, to_float(z[j]));
-        m = block_max(m, s_red);
-        if (m == -CUDART_INF_F) m = 0.0f;
-        float in = 0.0f, out = 0.0f;
-        for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-            const float e = pow2(exponent(to_float(z[j]), m, c));
-            bool taught = false;
-            for (uint32_t t = 0; rest && t < k; ++t) taught |= s_id[t] == static_cast<int32_t>(j);
-            if (taught)
-                in += e;
-            else
-                out += e;
-        }
-        in = block_sum(in, s_red);
-        out = block_sum(out, s_red);
-        const float sum = in + out;
-        const bool empty = sum == 0.0f || !taught_at_all;
-        const float log_s = logf(sum), inv_s = 1.0f / sum;
-        const float w = a.weight != nullptr ? a.weight[i] : 1.0f;
-        float r = rest && out > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
-        float term = 0.0f;
-        if (q > 0.0f || q != q) term = q * (log_q - ((to_float(z[id]) - m) * a.inv_t - log_s));
-        float loss = block_sum(term, s_red);
-        if (r > 0.0f) loss += r * (logf(r) - (logf(out) - log_s));
-        held += r;
-        const float pull = r > 0.0f ? r / (out * inv_s) : 0.0f;
-        if (threadIdx.x == 0 && a.loss != nullptr) a.loss[i] = empty ? 0.0f : loss * w;
-        const uint64_t to = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
-        for (uint32_t j = threadIdx.x; j < n && (a.grad != nullptr || a.hess != nullptr); j += kThreads) {
-            const float p = empty ? 0.0f : pow2(exponent(to_float(z[j]), m, c)) * inv_s;
-            float teach = 0.0f;
-            bool taught = false;
-            for (uint32_t t = 0; t < k; ++t)
-                if (s_id[t] == static_cast<int32_t>(j)) {
-                    teach += s_q[t];
-                    taught = true;
+            for (uint32_t k = 0; k < a.t.top; ++k)
+                if (s.id[k] == id[u] && k != u * 32 + lane) {
+                    only = false;
+                    if (k < u * 32 + lane) first_one = false;
                 }
-            float g = (taught ? held * p - teach : (held - pull) * p) * (w * a.inv_t);
-            float h = held * p * (1.0f - p) * (w * a.inv_t * a.inv_t);
-            if (empty) g = h = 0.0f;
-            if (a.row_weight != nullptr) {
-                g *= a.row_weight[first + j];
-                h *= a.row_weight[first + j];
-            }
-            most_g = fmaxf(most_g, fabsf(g));
-            most_h = fmaxf(most_h, fabsf(h));
-            if (a.grad != nullptr) static_cast<T*>(a.grad)[to + j] = from_float<T>(g);
-            if (a.hess != nullptr) static_cast<T*>(a.hess)[to + j] = from_float<T>(h);
         }
-        __syncthreads();  // the teacher's entries are read before the next list's are written
+        leads |= first_one ? 1u << u : 0u;
+        alone |= only ? 1u << u : 0u;
+        if (rest && first_one) top_sum += pow2(exponent(zt[u], m, c));
+        if (!rest && id[u] >= 0) total += expf(y[u] - y_max);
     }
-    if (a.max_g != nullptr) {
-        most_g = block_max(most_g, s_red);
-        most_h = block_max(most_h, s_red);
-        if (threadIdx.x == 0) {  // non-negative doubles order like their bit patterns
-            atomicMax(a.max_g, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(most_g))));
-            atomicMax(a.max_h, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(most_h))));
+    const float outside = warp_sum(sum);
+    if (rest) {
+        top_sum = warp_sum(top_sum);
+    } else {
+        total = warp_sum(total);
+    }
+    sum = outside + top_sum;
+    const float log_total = logf(total), log_sum = rest ? a.t.log_sum[i] : 0.0f;
+    float held = 0.0f, cross = 0.0f, q[kTop];
+#pragma unroll
+    for (int u = 0; u < kTop; ++u) {
+        float log_q = -CUDART_INF_F;
+        if (id[u] >= 0) log_q = rest ? y[u] - log_sum : total == 0.0f ? -CUDART_INF_F : y[u] - y_max - log_total;
+        q[u] = expf(log_q);
+        held += q[u];
+        if (q[u] != 0.0f) cross += q[u] * (log_q - (zt[u] - m) * a.inv_t);
+        if (u * 32 + lane < a.t.top) s.q[u * 32 + lane] = q[u];
+    }
+    held = warp_sum(held);
+    const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+    const bool empty = sum == 0.0f || !taught;
+    const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
+    if (a.loss != nullptr) {
+        cross = warp_sum(cross);
+        if (lane == 0) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+    }
+    if (a.grad == nullptr && a.hess == nullptr) return;
+    const Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
+    const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        const uint32_t j = u * 32 + lane;
+        const float p = x[u] * k.inv_s;
+        if (j < n)
+            put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * x[u], empty ? 0.0f : k.curve * p * (1.0f - p),
+                   ((marks >> u) & 1u) == 0, most);
+    }
+    __syncwarp();  // the top's own go over them
+#pragma unroll
+    for (int u = 0; u < kTop; ++u) {
+        if (((leads >> u) & 1u) == 0 || empty) continue;
+        float taught_q = q[u];
+        if (((alone >> u) & 1u) == 0) {
+            taught_q = 0.0f;
+            for (uint32_t e = 0; e < a.t.top; ++e)
+                if (s.id[e] == id[u]) taught_q += s.q[e];
         }
+        const float e = pow2(exponent(zt[u], m, c)), p = e * k.inv_s;
+        put<T>(a, out + id[u], first + id[u], k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p * (1.0f - p), true, most);
     }
+}
+
+// A warp per list; a longer one among them by the whole CTA.
+template <class T, int kTop>
+__global__ void __launch_bounds__(kWarpThreads) distill_warps_kernel(DistillArgs a) {
+    if (a.stopped != nullptr && *a.stopped) return;
+    constexpr uint32_t kLists = kWarpThreads / 32;
+    __shared__ WarpShared warps[kLists];
+    __shared__ Shared<kWarpThreads, kWarpThreads> shared;
+    const uint32_t base = blockIdx.x * kLists, i = base + (threadIdx.x >> 5);
+    uint64_t first = 0;
+    uint32_t n = 0;
+    Maxima most;
+    if (i < a.l.lists) {
+        list_range(a.l, i, first, n);
+        WarpShared& s = warps[threadIdx.x >> 5];
+        if (n <= 128)
+            distill_warp<T, 4, kTop>(s, a, i, first, n, most);
+        else if (n <= 256)
+            distill_warp<T, 8, kTop>(s, a, i, first, n, most);
+        else if (n <= kWarpEntries)
+            distill_warp<T, 16, kTop>(s, a, i, first, n, most);
+    }
+    if (__syncthreads_or(n > kWarpEntries) != 0)
+        for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
+            list_range(a.l, k, first, n);
+            if (n <= kWarpEntries) continue;
+            distill_list<T, 1, 1, kWarpThreads, false>(shared, a, k, 0, 1, most);
+            __syncthreads();
+        }
+    publish<kWarpThreads>(a, most);
+}
+
+template <class T, int kVec, int kHeld, int kThreads>
+void launch_rows(const DistillArgs& a, uint32_t shares, cudaStream_t s) {
+    if (shares == 1) {
+        distill_rows_kernel<T, kVec, kHeld, kThreads, false><<<a.l.lists, kThreads, 0, s>>>(a, 1);
+        return;
+    }
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.l.lists * shares);
+    config.blockDim = dim3(kThreads);
+    config.stream = s;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = shares;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, distill_rows_kernel<T, kVec, kHeld, kThreads, true>, a, shares);
+}
+
+template <class T>
+void launch_typed(const DistillArgs& a, cudaStream_t s) {
+    constexpr int kVec = 16 / sizeof(T), kHeld = 8;
+    const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
+    if (mean <= (a.l.bounds != nullptr ? kWarpEntries / 2 : kWarpEntries)) {
+        const uint32_t lists = kWarpThreads / 32, grid = (a.l.lists + lists - 1) / lists;
+        if (a.t.top <= 32)
+            distill_warps_kernel<T, 1><<<grid, kWarpThreads, 0, s>>>(a);
+        else
+            distill_warps_kernel<T, 4><<<grid, kWarpThreads, 0, s>>>(a);
+        return;
+    }
+    uint32_t shares = list_shares(mean, a.l.lists, a.sms);
+    if (a.l.bounds != nullptr) {
+        launch_rows<T, 1, 16, 512>(a, shares, s);
+        return;
+    }
+    // As many shares as hold the list in registers (8 at most, past which it is read again).
+    while (shares < 8 && mean > static_cast<uint64_t>(shares) * kVec * kHeld * 512) shares *= 2;
+    if (mean <= shares * kVec * kHeld * 128)
+        launch_rows<T, kVec, kHeld, 128>(a, shares, s);
+    else if (mean <= shares * kVec * kHeld * 256)
+        launch_rows<T, kVec, kHeld, 256>(a, shares, s);
+    else
+        launch_rows<T, kVec, kHeld, 512>(a, shares, s);
 }
 
 }  // namespace
 
 void launch_distill(const DistillArgs& a, cudaStream_t s) {
-    const uint32_t most = a.sms * 8, grid = a.l.lists < most ? a.l.lists : most;
     if (a.l.type == SB2_F32)
-        distill_kernel<float><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<float>(a, s);
     else if (a.l.type == SB2_BF16)
-        distill_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<__nv_bfloat16>(a, s);
     else
-        distill_kernel<__half><<<grid, kThreads, 0, s>>>(a);
+        launch_typed<__half>(a, s);
 }
 
 }  // namespace sb2
