@@ -12,8 +12,11 @@
 // others are, over what the common formula left there. An entry named twice has its q added in the teacher's order.
 //
 // Lists of at most kWarpEntries take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
-// holds it in registers between the sums and the gradients, so that memory sees each score once. A list too long for
-// that (or of scores so far from 0 that fma(z, c, -m c) loses its last bits) is read again for each pass.
+// holds it in shared memory between the passes (each thread its own vectors), so that memory sees each score once; runs
+// between boundaries are read again from the caches, entry by entry, so that a list's sums do not depend on where it
+// starts. A dense list too long for shared memory (or of scores so far from 0 that fma(z, c, -m c) loses its last bits) is read again for each
+// pass.
+#include <algorithm>
 #include <cfloat>
 
 #include "lists_device.cuh"
@@ -26,32 +29,36 @@ namespace {
 
 constexpr uint32_t kWarpEntries = 512;
 constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
+constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
+constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
 constexpr float kFar = 1048576.0f;   // |m c| from which an exponent is taken from the distance z - m
 
-// What a CTA keeps of its share of a list; kBits entries have a bit of their own, more share them.
-template <int kThreads, int kBits>
+constexpr uint32_t kBits = 65536;    // marks of a share: entries past so many share them
+
+// What a CTA keeps of its share of a list beside the scores.
+template <int kThreads>
 struct Shared {
-    float warp[7][kThreads / 32];
+    float warp[6][kThreads / 32];
     float m, outside;                // the share's reference, and its sum (outside the top, where the rest counts)
-    int32_t id[kMaxTop];
+    __align__(16) int32_t id[kMaxTop];
     float q[kMaxTop];
     uint32_t edge_bits;              // marks of the scalars outside the vectors
-    uint32_t bits[kBits / 32];
 };
 
+// The sum and the maximum of the warps' parts, in every thread.
 template <int kThreads>
 __device__ __forceinline__ float sum_of(const float (&part)[kThreads / 32]) {
-    float v = part[0];
+    float v = part[threadIdx.x & (kThreads / 32 - 1)];
 #pragma unroll
-    for (int k = 1; k < kThreads / 32; ++k) v += part[k];
+    for (int o = kThreads / 64; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
 
 template <int kThreads>
 __device__ __forceinline__ float max_of(const float (&part)[kThreads / 32]) {
-    float v = part[0];
+    float v = part[threadIdx.x & (kThreads / 32 - 1)];
 #pragma unroll
-    for (int k = 1; k < kThreads / 32; ++k) v = fmaxf(v, part[k]);
+    for (int o = kThreads / 64; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
 
@@ -92,8 +99,12 @@ __device__ __forceinline__ void publish(const DistillArgs& a, Maxima most) {
     }
     __syncthreads();
     if (threadIdx.x == 0) {  // non-negative doubles order like their bit patterns
-        atomicMax(a.max_g, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(max_of<kThreads>(s_g)))));
-        atomicMax(a.max_h, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(max_of<kThreads>(s_h)))));
+        for (int k = 1; k < kThreads / 32; ++k) {
+            most.g = fmaxf(most.g, s_g[k]);
+            most.h = fmaxf(most.h, s_h[k]);
+        }
+        atomicMax(a.max_g, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(most.g))));
+        atomicMax(a.max_h, static_cast<unsigned long long>(__double_as_longlong(static_cast<double>(most.h))));
     }
 }
 
@@ -144,31 +155,30 @@ __device__ __forceinline__ Slopes slopes_of(float w, float inv_t, float held, fl
     return k;
 }
 
-// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). kHeld vectors a thread
-// stay in registers.
-template <class T, int kVec, int kHeld, int kThreads, bool kCluster>
-__device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kThreads>& s, const DistillArgs& a, uint32_t i,
-                                             uint32_t share, uint32_t shares, Maxima& most) {
-    constexpr uint32_t kBits = kVec * kHeld * kThreads;
+// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). `data` holds `slots` vectors
+// (scores, for kVec 1), then the marks: where the share is no longer, it stays there.
+template <class T, int kVec, int kThreads, bool kCluster>
+__device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>* data, uint32_t slots, uint32_t* bits,
+                                             const DistillArgs& a, uint32_t i, uint32_t share, uint32_t shares, Maxima& most) {
+    constexpr int kUnroll = kVec == 1 ? 4 : 2;
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
     uint64_t first;
     uint32_t n;
     list_range(a.l, i, first, n);
     const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
-    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * share / shares);
-    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * (share + 1) / shares);
+    uint32_t from = 0, to = w.vectors;
+    if constexpr (kCluster) {  // shares is a power of two
+        const uint32_t shift = __ffs(shares) - 1;
+        from = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * share) >> shift);
+        to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
+    }
     const float c = __fmul_rn(kLog2E, a.inv_t);
     const bool rest = a.t.log_sum != nullptr, marks = rest || a.max_g != nullptr;
-    const bool held_here = to - from <= kHeld * kThreads;
-    // The scores, on their way.
-    Pack<T, kVec> p[kHeld];
-#pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-        const uint32_t v = from + u * kThreads + t;
-        if (held_here && v < to)
-            p[u].load(w.z + w.at(v));
-        else
-            p[u].masked();
+    const bool held_here = kVec == 1 || to - from <= slots;
+    // The scores, on their way to the thread's own slots.
+    if (kVec > 1 && held_here) {
+        for (uint32_t v = from + t; v < to; v += kThreads) data[v - from].copy(w.z + w.at(v));
+        copies_begun();
     }
     const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
     const float edge = edge_at < n ? to_float(w.z[edge_at]) : -CUDART_INF_F;
@@ -178,11 +188,11 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
     if (t < a.t.top) {
         teacher_entry(a, i, t, n, id, y);
         if (id >= 0) zt = to_float(w.z[id]);
-        s.id[t] = id;
     }
+    if (t < kMaxTop) s.id[t] = id;
     if (marks) {
-        const uint32_t words = min(kBits, (to - from) * kVec + 31) / 32;
-        for (uint32_t k = t; k < words; k += kThreads) s.bits[k] = 0;
+        const uint32_t words = held_here ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
+        for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
         if (t == 0) s.edge_bits = 0;
         __syncthreads();
         if (id >= 0) {
@@ -191,15 +201,25 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
                 atomicOr(&s.edge_bits, 1u << (j < w.head ? j : w.head + (j - w.tail())));
             } else if ((j - w.head) / kVec >= from && (j - w.head) / kVec < to) {
                 const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
-                atomicOr(&s.bits[bit / 32], 1u << (bit & 31));
+                if (held_here) atomicOr(&bits[bit / 32], 1u << (bit & 31));
             }
         }
     }
-    // Marks of vector `v`'s entries. Entries that share bits (a list too long for the registers) look among the ids.
+    // Vector `v` of the share; a run between boundaries, entry by entry, is read from its place each time.
+    auto get = [&](uint32_t v, float(&x)[kVec]) {
+        if constexpr (kVec == 1)
+            x[0] = to_float(__ldg(w.z + from + v));
+        else
+            data[v].values(x);
+    };
+    // Marks of vector `v`'s entries. Where the marks are shared or there are none, the ids themselves decide.
     auto marked = [&](uint32_t v) {
-        const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
-        uint32_t m = (s.bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
-        if (!held_here && m != 0) {
+        uint32_t m = ~0u;
+        if (held_here) {
+            const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
+            m = (bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
+        }
+        if (m != 0 && (!held_here || (to - from) * kVec > kBits)) {
             m = 0;
             for (uint32_t k = 0; k < a.t.top; ++k) {
                 const uint32_t e = static_cast<uint32_t>(s.id[k]) - w.at(v);
@@ -210,14 +230,18 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
     };
     // The maxima of the scores and of the teacher's.
     float m = fmaxf(edge, zt);  // with the top's scores, so that no share's reference lies far below them
-    if (held_here) {
+    if constexpr (kVec == 1) {
+#pragma unroll 4
+        for (uint32_t v = t; v < to - from; v += kThreads) m = fmaxf(m, to_float(__ldg(w.z + from + v)));
+    } else if (held_here) {
+        Pack<T, kVec> top;
+        top.masked();
+        copies_done();
+        for (uint32_t v = t; v < to - from; v += kThreads) top.raise(data[v]);
+        float x[kVec];
+        top.values(x);
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            float x[kVec];
-            p[u].values(x);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) m = fmaxf(m, x[e]);
-        }
+        for (int e = 0; e < kVec; ++e) m = fmaxf(m, x[e]);
     } else {
         for (uint32_t v = from + t; v < to; v += kThreads) {
             Pack<T, kVec> now;
@@ -243,28 +267,31 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
     if (!far) {
         const float2 cc = make_float2(c, c), minus_r = make_float2(-R, -R);
         float2 two = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            const uint32_t v = from + u * kThreads + t;
-            if (v >= to) break;
+        auto add = [&](uint32_t v, bool look) {
             float x[kVec];
-            p[u].values(x);
-            if constexpr (kVec == 1) {
-                const float e = pow2(__fmaf_rn(x[0], c, -R));
-                if (!rest || marked(v) == 0) sum += e;
-            } else {
-                const uint32_t skip = rest ? marked(v) : 0;
-                if (skip != 0) {
+            get(v, x);
+            const uint32_t skip = look ? marked(from + v) : 0;
+            if (skip != 0) {
 #pragma unroll
-                    for (int e = 0; e < kVec; ++e)
-                        if ((skip >> e) & 1u) x[e] = -CUDART_INF_F;
-                }
+                for (int e = 0; e < kVec; ++e)
+                    if ((skip >> e) & 1u) x[e] = -CUDART_INF_F;
+            }
+            if constexpr (kVec == 1) {
+                sum += pow2(__fmaf_rn(x[0], c, -R));
+            } else {
 #pragma unroll
                 for (int e = 0; e < kVec; e += 2) {
                     const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), cc, minus_r);
                     two = __fadd2_rn(two, make_float2(pow2(z.x), pow2(z.y)));
                 }
             }
+        };
+        if (rest) {
+#pragma unroll kUnroll
+            for (uint32_t v = t; v < to - from; v += kThreads) add(v, true);
+        } else {
+#pragma unroll kUnroll
+            for (uint32_t v = t; v < to - from; v += kThreads) add(v, false);
         }
         sum += two.x + two.y;
     } else {
@@ -281,31 +308,45 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
     auto term = [&](float z) { return far ? pow2(exponent(z, m, c)) : pow2(__fmaf_rn(z, c, -R)); };
     const bool edge_marked = marks && edge_at < n && ((s.edge_bits >> t) & 1u) != 0;
     if (edge_at < n && !(rest && edge_marked)) sum += term(edge);
-    bool leads = id >= 0, alone = true;
+    bool leads = id >= 0, alone = true;  // the first of the teacher's entries that names this index, and the only one
     if (t < a.t.top) {
-        for (uint32_t k = 0; k < a.t.top; ++k)
-            if (s.id[k] == id && k != t) {
-                alone = false;
-                if (k < t) leads = false;
+        uint32_t same = 0, before = 0;
+        for (uint32_t k = 0; k < a.t.top; k += 4) {  // (s.id is -1 up to the next multiple of 4)
+            const int4 o = *reinterpret_cast<const int4*>(&s.id[k]);
+            const uint32_t hit = (o.x == id ? 1u : 0u) | (o.y == id ? 2u : 0u) | (o.z == id ? 4u : 0u) | (o.w == id ? 8u : 0u);
+            if (hit != 0) {
+                same += __popc(hit);
+                before += __popc(k > t ? 0u : hit & ((1u << (t - k < 4 ? t - k : 4)) - 1u));
             }
+        }
+        alone = same == 1;
+        leads = leads && before == 0;
     }
-    const float e_t = id >= 0 ? term(zt) : 0.0f;
-    float top_sum = rest && leads ? e_t : 0.0f;
-    float total = rest || id < 0 ? 0.0f : expf(y - y_max);
+    // The teacher's terms, not yet divided by their sum where the top is all of it.
+    const float base = rest ? a.t.log_sum[i] : y_max;
+    float q = id >= 0 ? expf(y - base) : 0.0f;
     sum = warp_sum(sum);
-    top_sum = warp_sum(top_sum);
-    total = warp_sum(total);
-    if (lane == 0) {
-        s.warp[2][warp] = sum;
-        s.warp[3][warp] = top_sum;
-        s.warp[4][warp] = total;
+    if (lane == 0) s.warp[2][warp] = sum;
+    if (warp * 32 < a.t.top) {
+        s.q[t] = q;
+        const float top_part = warp_sum(rest && leads ? term(zt) : 0.0f);
+        const float held_part = warp_sum(q);
+        const float cross_part = warp_sum(q != 0.0f ? q * (y - base - (zt - m) * a.inv_t) : 0.0f);
+        if (lane == 0) {
+            s.warp[3][warp] = top_part;
+            s.warp[4][warp] = held_part;
+            s.warp[5][warp] = cross_part;
+        }
+    } else if (lane == 0) {
+        s.warp[3][warp] = s.warp[4][warp] = s.warp[5][warp] = 0.0f;
     }
     __syncthreads();
     // About m itself: the rounding of R is put back.
     const float settle = far ? 1.0f : pow2(-__fmaf_rn(m, c, -R));
     float outside = settle * sum_of<kThreads>(s.warp[2]);
-    top_sum = settle * sum_of<kThreads>(s.warp[3]);
-    total = sum_of<kThreads>(s.warp[4]);
+    float top_sum = settle * sum_of<kThreads>(s.warp[3]);
+    float held = sum_of<kThreads>(s.warp[4]);
+    float cross = sum_of<kThreads>(s.warp[5]);
     if constexpr (kCluster) {
         // Every share's sum is about its own reference: their sum is about the largest.
         cg::cluster_group cluster = cg::this_cluster();
@@ -322,32 +363,29 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
             joined += other->outside * pow2(exponent(other->m, all, c));
         }
         outside = joined;
+        cluster.barrier_arrive();  // the shares' memory is read
         top_sum *= pow2(exponent(m, all, c));
+        cross += held * ((all - m) * a.inv_t);
         m = all;
         R = __fmul_rn(m, c);
         far = !(fabsf(R) < kFar) || !held_here;
-        cluster.sync();  // the shares' memory is read
     }
     sum = outside + top_sum;
-    // The teacher's q, and the loss.
-    float log_q = -CUDART_INF_F;
-    if (id >= 0) log_q = rest ? y - a.t.log_sum[i] : total == 0.0f ? -CUDART_INF_F : y - y_max - logf(total);
-    const float q = expf(log_q);
-    if (t < a.t.top) s.q[t] = q;
-    float held = warp_sum(q);
-    float cross = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
-    if (lane == 0) {
-        s.warp[5][warp] = held;
-        s.warp[6][warp] = cross;
+    float q_scale = 1.0f;
+    if (!rest && held != 0.0f) {
+        q_scale = 1.0f / held;
+        cross = cross * q_scale - logf(held);
+        held = 1.0f;
     }
-    __syncthreads();
-    held = sum_of<kThreads>(s.warp[5]);
-    cross = sum_of<kThreads>(s.warp[6]);
+    q *= q_scale;
     const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
     const bool empty = sum == 0.0f || !taught;
     const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
     if (t == 0 && share == 0 && a.loss != nullptr) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
-    if (a.grad == nullptr && a.hess == nullptr) return;
+    if (a.grad == nullptr && a.hess == nullptr) {
+        if constexpr (kCluster) cg::this_cluster().barrier_wait();
+        return;
+    }
     // The derivatives outside the top, and what the same formula gives in it.
     Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
     if (!far) {  // the terms are about R
@@ -362,43 +400,60 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
         put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * e, empty ? 0.0f : k.curve * q_j * (1.0f - q_j), counts, most);
     };
     if (!far && !empty) {
-        T* const grad = a.grad != nullptr ? static_cast<T*>(a.grad) + out : nullptr;
-        T* const hess = a.hess != nullptr ? static_cast<T*>(a.hess) + out : nullptr;
-        const bool aligned = kVec > 1 && ((reinterpret_cast<uintptr_t>(grad + w.head) | reinterpret_cast<uintptr_t>(hess + w.head)) & 15) == 0;
+        T* const grad = a.grad != nullptr ? static_cast<T*>(a.grad) + out + w.at(from) : nullptr;
+        T* const hess = a.hess != nullptr ? static_cast<T*>(a.hess) + out + w.at(from) : nullptr;
+        const bool aligned = ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(hess)) & 15) == 0;
         const float2 cc = make_float2(c, c), minus_r = make_float2(-R, -R), slope = make_float2(k.slope, k.slope);
+        if (kVec == 1 && (a.max_g != nullptr || a.row_weight != nullptr)) {
+#pragma unroll 4
+            for (uint32_t v = t; v < to - from; v += kThreads) {
+                float x[kVec];
+                get(v, x);
+                put_one(x[0], w.at(from + v), a.max_g == nullptr || marked(from + v) == 0);
+            }
+        } else if (kVec == 1) {
+#pragma unroll 4
+            for (uint32_t v = t; v < to - from; v += kThreads) {
+                float x[kVec];
+                get(v, x);
+                const float e = pow2(__fmaf_rn(x[0], c, -R)), p_j = e * k.inv_s;
+                if (grad != nullptr) grad[v] = from_float<T>(k.slope * e);
+                if (hess != nullptr) hess[v] = from_float<T>(k.curve * p_j * (1.0f - p_j));
+            }
+        } else if (kVec > 1 && aligned && grad != nullptr && hess == nullptr) {
+#pragma unroll 2
+            for (uint32_t v = t; v < to - from; v += kThreads) {
+                float x[kVec];
+                get(v, x);
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            const uint32_t v = from + u * kThreads + t;
-            if (v >= to) break;
-            float x[kVec];
-            p[u].values(x);
-            if constexpr (kVec == 1) {
-                put_one(x[0], w.at(v), a.max_g == nullptr || marked(v) == 0);
-            } else {
-                float g[kVec], h[kVec];
-#pragma unroll
-                for (int e = 0; e < kVec; e += 2) {
+                for (int e = 0; e + 1 < kVec; e += 2) {
                     const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), cc, minus_r);
-                    const float2 two = __fmul2_rn(make_float2(x[e] = pow2(z.x), x[e + 1] = pow2(z.y)), slope);
-                    g[e] = two.x;
-                    g[e + 1] = two.y;
+                    const float2 g = __fmul2_rn(make_float2(pow2(z.x), pow2(z.y)), slope);
+                    x[e] = g.x;
+                    x[e + 1] = g.y;
                 }
-                if (hess != nullptr) {
+                if constexpr (kVec > 1) __stcs(reinterpret_cast<uint4*>(grad) + v, packed<T, kVec>(x));
+            }
+        } else {
+            for (uint32_t v = t; v < to - from; v += kThreads) {
+                float x[kVec], g[kVec], h[kVec];
+                get(v, x);
 #pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        const float q_j = x[e] * k.inv_s;
-                        h[e] = k.curve * q_j * (1.0f - q_j);
-                    }
+                for (int e = 0; e < kVec; ++e) {
+                    const float z = pow2(__fmaf_rn(x[e], c, -R)), p_j = z * k.inv_s;
+                    g[e] = k.slope * z;
+                    h[e] = k.curve * p_j * (1.0f - p_j);
                 }
-                const uint32_t j = w.at(v);
-                if (aligned) {
-                    if (grad != nullptr) __stcs(reinterpret_cast<uint4*>(grad + j), packed<T, kVec>(g));
-                    if (hess != nullptr) __stcs(reinterpret_cast<uint4*>(hess + j), packed<T, kVec>(h));
+                if (kVec > 1 && aligned) {
+                    if constexpr (kVec > 1) {
+                        if (grad != nullptr) __stcs(reinterpret_cast<uint4*>(grad) + v, packed<T, kVec>(g));
+                        if (hess != nullptr) __stcs(reinterpret_cast<uint4*>(hess) + v, packed<T, kVec>(h));
+                    }
                 } else {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
-                        if (grad != nullptr) grad[j + e] = from_float<T>(g[e]);
-                        if (hess != nullptr) hess[j + e] = from_float<T>(h[e]);
+                        if (grad != nullptr) grad[v * kVec + e] = from_float<T>(g[e]);
+                        if (hess != nullptr) hess[v * kVec + e] = from_float<T>(h[e]);
                     }
                 }
             }
@@ -421,21 +476,25 @@ __device__ __forceinline__ void distill_list(Shared<kThreads, kVec * kHeld * kTh
             if (!alone) {
                 taught_q = 0.0f;
                 for (uint32_t x = 0; x < a.t.top; ++x)
-                    if (s.id[x] == id) taught_q += s.q[x];
+                    if (s.id[x] == id) taught_q += s.q[x] * q_scale;
             }
             const float e = term(zt), p_j = e * k.inv_s;
             put<T>(a, out + j, first + j, k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p_j * (1.0f - p_j), true, most);
         }
     }
+    if constexpr (kCluster) cg::this_cluster().barrier_wait();
 }
 
-template <class T, int kVec, int kHeld, int kThreads, bool kCluster>
-__global__ void __launch_bounds__(kThreads, kVec == 1 ? 1 : 1024 / kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares) {
+template <class T, int kVec, int kThreads, bool kCluster>
+__global__ void __launch_bounds__(kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares, uint32_t slots) {
     if (a.stopped != nullptr && *a.stopped) return;
-    __shared__ Shared<kThreads, kVec * kHeld * kThreads> s;
+    extern __shared__ __align__(16) unsigned char held[];
+    __shared__ Shared<kThreads> s;
     Maxima most;
-    const uint32_t i = kCluster ? blockIdx.x / shares : blockIdx.x;
-    distill_list<T, kVec, kHeld, kThreads, kCluster>(s, a, i, kCluster ? blockIdx.x % shares : 0, kCluster ? shares : 1, most);
+    Pack<T, kVec>* data = reinterpret_cast<Pack<T, kVec>*>(held);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(held + ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)));
+    const uint32_t shift = kCluster ? __ffs(shares) - 1 : 0;
+    distill_list<T, kVec, kThreads, kCluster>(s, data, slots, bits, a, blockIdx.x >> shift, blockIdx.x & (shares - 1), shares, most);
     publish<kThreads>(a, most);
 }
 
@@ -573,7 +632,8 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warps_kernel(DistillArgs
     if (a.stopped != nullptr && *a.stopped) return;
     constexpr uint32_t kLists = kWarpThreads / 32;
     __shared__ WarpShared warps[kLists];
-    __shared__ Shared<kWarpThreads, kWarpThreads> shared;
+    __shared__ Shared<kWarpThreads> shared;
+    __shared__ uint32_t bits[kBits / 32];
     const uint32_t base = blockIdx.x * kLists, i = base + (threadIdx.x >> 5);
     uint64_t first = 0;
     uint32_t n = 0;
@@ -592,34 +652,41 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warps_kernel(DistillArgs
         for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
             list_range(a.l, k, first, n);
             if (n <= kWarpEntries) continue;
-            distill_list<T, 1, 1, kWarpThreads, false>(shared, a, k, 0, 1, most);
+            distill_list<T, 1, kWarpThreads, false>(shared, nullptr, 0, bits, a, k, 0, 1, most);
             __syncthreads();
         }
     publish<kWarpThreads>(a, most);
 }
 
-template <class T, int kVec, int kHeld, int kThreads>
-void launch_rows(const DistillArgs& a, uint32_t shares, cudaStream_t s) {
-    if (shares == 1) {
-        distill_rows_kernel<T, kVec, kHeld, kThreads, false><<<a.l.lists, kThreads, 0, s>>>(a, 1);
-        return;
-    }
+// Shared memory of a CTA that holds `slots` vectors and their marks.
+template <class T, int kVec>
+size_t rows_smem(uint32_t slots) {
+    if (kVec == 1) return kBits / 8;
+    const size_t entries = static_cast<size_t>(slots) * kVec;
+    return ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)) + (std::min<size_t>(entries, kBits) + 31) / 32 * 4;
+}
+
+template <class T, int kVec, int kThreads>
+void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStream_t s) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(a.l.lists * shares);
     config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = rows_smem<T, kVec>(slots);
     config.stream = s;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = shares;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
-    config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, distill_rows_kernel<T, kVec, kHeld, kThreads, true>, a, shares);
+    config.numAttrs = shares > 1 ? 1 : 0;
+    auto* kernel = shares > 1 ? distill_rows_kernel<T, kVec, kThreads, true> : distill_rows_kernel<T, kVec, kThreads, false>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHeld) != cudaSuccess) return;
+    cudaLaunchKernelEx(&config, kernel, a, shares, slots);
 }
 
 template <class T>
 void launch_typed(const DistillArgs& a, cudaStream_t s) {
-    constexpr int kVec = 16 / sizeof(T), kHeld = 8;
+    constexpr int kVec = 16 / sizeof(T);
     const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
     if (mean <= (a.l.bounds != nullptr ? kWarpEntries / 2 : kWarpEntries)) {
         const uint32_t lists = kWarpThreads / 32, grid = (a.l.lists + lists - 1) / lists;
@@ -631,17 +698,21 @@ void launch_typed(const DistillArgs& a, cudaStream_t s) {
     }
     uint32_t shares = list_shares(mean, a.l.lists, a.sms);
     if (a.l.bounds != nullptr) {
-        launch_rows<T, 1, 16, 512>(a, shares, s);
+        if (mean / shares <= 1024)
+            launch_rows<T, 1, 128>(a, shares, 0, s);
+        else
+            launch_rows<T, 1, 256>(a, shares, 0, s);
         return;
     }
-    // As many shares as hold the list in registers (8 at most, past which it is read again).
-    while (shares < 8 && mean > static_cast<uint64_t>(shares) * kVec * kHeld * 512) shares *= 2;
-    if (mean <= shares * kVec * kHeld * 128)
-        launch_rows<T, kVec, kHeld, 128>(a, shares, s);
-    else if (mean <= shares * kVec * kHeld * 256)
-        launch_rows<T, kVec, kHeld, 256>(a, shares, s);
+    // As many shares as hold the list in kHeld bytes each, else in kMaxHeld (longer: read again).
+    const uint64_t bytes = mean * sizeof(T);
+    while (shares < 8 && bytes > static_cast<uint64_t>(shares) * kHeld) shares *= 2;
+    uint64_t slots = (mean / kVec + shares - 1) / shares;
+    if (rows_smem<T, kVec>(static_cast<uint32_t>(std::min<uint64_t>(slots, kMaxHeld / 16))) > kMaxHeld) slots = 0;
+    if (mean / shares <= 4096)
+        launch_rows<T, kVec, 128>(a, shares, static_cast<uint32_t>(slots), s);
     else
-        launch_rows<T, kVec, kHeld, 512>(a, shares, s);
+        launch_rows<T, kVec, 256>(a, shares, static_cast<uint32_t>(slots), s);
 }
 
 }  // namespace

@@ -109,6 +109,11 @@ template <class T, int kVec>
 struct Pack {
     uint4 raw;
     __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
+    // Into shared memory, without a register (copies_done() waits for the thread's own).
+    __device__ __forceinline__ void copy(const T* p) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(this))), "l"(p)
+                     : "memory");
+    }
     __device__ __forceinline__ void values(float (&f)[kVec]) const {
         if constexpr (sizeof(T) == 4) {
             f[0] = __uint_as_float(raw.x);
@@ -130,6 +135,29 @@ struct Pack {
             }
         }
     }
+    // The larger of each entry and its counterpart (a NaN gives way).
+    __device__ __forceinline__ void raise(const Pack& o) {
+        if constexpr (sizeof(T) == 4) {
+            raw.x = __float_as_uint(fmaxf(__uint_as_float(raw.x), __uint_as_float(o.raw.x)));
+            raw.y = __float_as_uint(fmaxf(__uint_as_float(raw.y), __uint_as_float(o.raw.y)));
+            raw.z = __float_as_uint(fmaxf(__uint_as_float(raw.z), __uint_as_float(o.raw.z)));
+            raw.w = __float_as_uint(fmaxf(__uint_as_float(raw.w), __uint_as_float(o.raw.w)));
+        } else {
+            raw.x = larger(raw.x, o.raw.x);
+            raw.y = larger(raw.y, o.raw.y);
+            raw.z = larger(raw.z, o.raw.z);
+            raw.w = larger(raw.w, o.raw.w);
+        }
+    }
+    __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&m);
+        } else {
+            const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&m);
+        }
+    }
     __device__ __forceinline__ void masked() {  // every entry -inf
         const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, __nv_bfloat16> ? 0xFF80FF80u : 0xFC00FC00u;
         raw = make_uint4(w, w, w, w);
@@ -139,9 +167,20 @@ template <class T>
 struct Pack<T, 1> {
     T raw;
     __device__ __forceinline__ void load(const T* p) { raw = __ldg(p); }
+    __device__ __forceinline__ void copy(const T* p) {
+        if constexpr (sizeof(T) == 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(this))), "l"(p)
+                         : "memory");
+        else
+            raw = __ldg(p);
+    }
     __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = to_float(raw); }
+    __device__ __forceinline__ void raise(const Pack& o) { raw = to_float(o.raw) > to_float(raw) || raw != raw ? o.raw : raw; }
     __device__ __forceinline__ void masked() { raw = from_float<T>(-CUDART_INF_F); }
 };
+
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
