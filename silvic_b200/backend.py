@@ -14,6 +14,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import _abi
+from . import lists as _lists
 from .dataset import BinnedDataset
 from .lists import Distilled, LogProbs, TeacherTop
 
@@ -265,27 +266,22 @@ class B200Backend:
         entries (int32 [lists, n] or [lists]), the entropy, the log sum and the `top` likeliest entries (at most 128).
         `scores`: a CUDA tensor, f32, bf16 or f16, of a list a row, or 1-D with `boundaries` (int32 or uint32, lists
         + 1). Runs on torch's current stream of the handle's device, without waiting; may be captured into a graph."""
-        import torch
-
-        from . import lists as L
-
-        arg = L.lists_arg(scores, boundaries)
+        arg = _lists.lists_arg(scores, boundaries)
         n = arg.num_lists
-        given = None if given is None else L.given_arg(given, n)
-        num_given = 0 if given is None else given.shape[1]
-        if not 0 <= top <= L.MAX_TOP:
-            raise ValueError(f"{top} alternatives; 0 to {L.MAX_TOP} are given")
-        L.check_device(self._device, [t for t in (scores, boundaries, given) if t is not None])
-        f32 = dict(dtype=torch.float32, device=scores.device)
-        out = LogProbs(torch.empty((n, num_given), **f32) if given is not None else None, torch.empty(n, **f32),
-                       torch.empty(n, **f32),
-                       torch.empty((n, top), dtype=torch.int32, device=scores.device) if top else None,
-                       torch.empty((n, top), **f32) if top else None)
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self._check(self._lib.sb2_log_probs(self._h, C.byref(arg), temperature, ptr(given), num_given, top,
-                                            ptr(out.given), ptr(out.entropy), ptr(out.log_sum), ptr(out.top_ids),
-                                            ptr(out.top), torch.cuda.current_stream(scores.device).cuda_stream))
-        return out
+        num_given = 0
+        if given is not None:
+            given = _lists.given_arg(given, n)
+            num_given = given.shape[1]
+        if not 0 <= top <= _lists.MAX_TOP:
+            raise ValueError(f"{top} alternatives; 0 to {_lists.MAX_TOP} are given")
+        _lists.check_device(self._device, (scores, boundaries, given))
+        # The outputs in one allocation, whose parts start at multiples of 4 bytes.
+        made = _lists.Outputs(scores, n, (num_given, 1, 1, top, top))
+        at = made.pointers
+        self._check(self._lib.sb2_log_probs(self._h, arg, temperature, given.data_ptr() if num_given else None, num_given,
+                                            top, at[0], at[1], at[2], at[3], at[4], _lists.stream(self._device)))
+        return LogProbs(made.part(0) if given is not None else None, made.flat(1), made.flat(2),
+                        made.ids(3) if top else None, made.part(4) if top else None)
 
     def distill(self, scores, teacher: TeacherTop, *, boundaries=None, weight=None, gradient: bool = True,
                 hessian: bool = False) -> Distilled:
@@ -294,38 +290,26 @@ class B200Backend:
         as in `log_probs`; `weight` (f32 [lists]) multiplies a list's loss and derivatives (a loss's upstream
         gradient, say). Gradient and hessian have the scores' type and shape, in memory of their own. Runs on torch's
         current stream of the handle's device, without waiting; may be captured into a graph."""
-        import torch
-
-        from . import lists as L
-
-        arg = L.lists_arg(scores, boundaries)
+        arg = _lists.lists_arg(scores, boundaries)
         n = arg.num_lists
-        t, keep = L.teacher_arg(teacher, n)
+        t, keep = _lists.teacher_arg(teacher, n)
         if weight is not None:
-            weight = L.per_list_arg(weight, n, "weight")
-        L.check_device(self._device, keep + [x for x in (scores, boundaries, weight) if x is not None])
+            weight = _lists.per_list_arg(weight, n, "weight")
+        _lists.check_device(self._device, (scores, boundaries, weight, *keep))
+        loss = scores.new_empty(n, dtype=_lists.torch_float32())
         # Gradients of padded rows are padded alike, so that both sides' rows start on the same boundaries; rows cut
         # from far wider ones (a stride of more than the width and 64) lie one behind the other.
         stride = 0 if boundaries is not None else arg.stride if arg.stride <= arg.width + 64 else arg.width
-
-        def empty():
-            if boundaries is not None or n == 0:
-                return torch.empty_like(scores, memory_format=torch.contiguous_format)
-            return torch.empty((n, stride), dtype=scores.dtype, device=scores.device)[:, : arg.width]
-
-        out = Distilled(torch.empty(n, dtype=torch.float32, device=scores.device), empty() if gradient else None,
-                        empty() if hessian else None)
-        ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-        self._check(self._lib.sb2_distill(self._h, C.byref(arg), C.byref(t), teacher.temperature, ptr(weight),
-                                          ptr(out.loss), ptr(out.gradient), ptr(out.hessian), stride,
-                                          torch.cuda.current_stream(scores.device).cuda_stream))
-        return out
+        grad = _lists.like(scores, n, arg.width, stride) if gradient else None
+        hess = _lists.like(scores, n, arg.width, stride) if hessian else None
+        self._check(self._lib.sb2_distill(self._h, arg, t, teacher.temperature, None if weight is None else weight.data_ptr(),
+                                          loss.data_ptr(), None if grad is None else grad.data_ptr(),
+                                          None if hess is None else hess.data_ptr(), stride, _lists.stream(self._device)))
+        return Distilled(loss, grad, hess)
 
     def set_teacher(self, teacher: TeacherTop):
         """sb2_set_teacher: the teacher of the loaded `distill` objective, a row of numpy arrays a query."""
-        from .lists import host_teacher
-
-        ids, logits, log_sum = host_teacher(teacher)
+        ids, logits, log_sum = _lists.host_teacher(teacher)
         f32 = lambda a: None if a is None else a.ctypes.data_as(C.POINTER(C.c_float))  # noqa: E731
         self._check(self._lib.sb2_set_teacher(self._h, ids.ctypes.data_as(C.POINTER(C.c_int32)), f32(logits),
                                               f32(log_sum), ids.shape[0], ids.shape[1], teacher.temperature))

@@ -39,9 +39,10 @@ constexpr uint32_t kBits = 65536;    // marks of a share: entries past so many s
 template <int kThreads>
 struct Shared {
     float warp[6][kThreads / 32];
-    float m, outside;                // the share's reference, and its sum (outside the top, where the rest counts)
+    float m, outside, top;           // the share's reference and sums (with the rest: outside the top, and in it)
     __align__(16) int32_t id[kMaxTop];
     float q[kMaxTop];
+    uint32_t again;                  // some entry's mark was set before
     uint32_t edge_bits;              // marks of the scalars outside the vectors
 };
 
@@ -173,7 +174,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
     }
     const float c = __fmul_rn(kLog2E, a.inv_t);
-    const bool rest = a.t.log_sum != nullptr, marks = rest || a.max_g != nullptr;
+    const bool rest = a.t.log_sum != nullptr;
     const bool held_here = kVec == 1 || to - from <= slots;
     // The scores, on their way to the thread's own slots.
     if (kVec > 1 && held_here) {
@@ -190,20 +191,25 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         if (id >= 0) zt = to_float(w.z[id]);
     }
     if (t < kMaxTop) s.id[t] = id;
-    if (marks) {
-        const uint32_t words = held_here ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
-        for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
-        if (t == 0) s.edge_bits = 0;
-        __syncthreads();
-        if (id >= 0) {
-            const uint32_t j = static_cast<uint32_t>(id);
-            if (j < w.head || j >= w.tail()) {
-                atomicOr(&s.edge_bits, 1u << (j < w.head ? j : w.head + (j - w.tail())));
-            } else if ((j - w.head) / kVec >= from && (j - w.head) / kVec < to) {
-                const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
-                if (held_here) atomicOr(&bits[bit / 32], 1u << (bit & 31));
-            }
+    const uint32_t words = held_here ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
+    for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
+    if (t == 0) s.edge_bits = s.again = 0;
+    __syncthreads();
+    bool mine = false;  // the entry lies in this share
+    if (id >= 0) {
+        const uint32_t j = static_cast<uint32_t>(id);
+        uint32_t before = 0, mark = 0;
+        if (j < w.head || j >= w.tail()) {
+            mine = share == 0;
+            mark = 1u << (j < w.head ? j : w.head + (j - w.tail()));
+            before = atomicOr(&s.edge_bits, mark);
+        } else if ((j - w.head) / kVec >= from && (j - w.head) / kVec < to) {
+            mine = true;
+            const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
+            mark = 1u << (bit & 31);
+            before = held_here ? atomicOr(&bits[bit / 32], mark) : mark;
         }
+        if ((before & mark) != 0) s.again = 1;  // an index named twice, or one that shares its mark
     }
     // Vector `v` of the share; a run between boundaries, entry by entry, is read from its place each time.
     auto get = [&](uint32_t v, float(&x)[kVec]) {
@@ -306,10 +312,10 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         }
     }
     auto term = [&](float z) { return far ? pow2(exponent(z, m, c)) : pow2(__fmaf_rn(z, c, -R)); };
-    const bool edge_marked = marks && edge_at < n && ((s.edge_bits >> t) & 1u) != 0;
+    const bool edge_marked = edge_at < n && ((s.edge_bits >> t) & 1u) != 0;
     if (edge_at < n && !(rest && edge_marked)) sum += term(edge);
-    bool leads = id >= 0, alone = true;  // the first of the teacher's entries that names this index, and the only one
-    if (t < a.t.top) {
+    bool leads = mine, alone = true;  // the first of the teacher's entries that names this index, and the only one
+    if (s.again != 0 && t < a.t.top) {
         uint32_t same = 0, before = 0;
         for (uint32_t k = 0; k < a.t.top; k += 4) {  // (s.id is -1 up to the next multiple of 4)
             const int4 o = *reinterpret_cast<const int4*>(&s.id[k]);
@@ -353,18 +359,25 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         if (t == 0) {
             s.m = m;
             s.outside = outside;
+            s.top = top_sum;
         }
         cluster.sync();
-        float all = -FLT_MAX;
-        for (uint32_t k = 0; k < shares; ++k) all = fmaxf(all, cluster.map_shared_rank(&s, k)->m);
-        float joined = 0.0f;
-        for (uint32_t k = 0; k < shares; ++k) {
-            const auto* other = cluster.map_shared_rank(&s, k);
-            joined += other->outside * pow2(exponent(other->m, all, c));
+        const auto* other = cluster.map_shared_rank(&s, lane & (shares - 1));
+        const float other_m = other->m, other_outside = other->outside, other_top = other->top;
+        float all = other_m;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFull, all, o));
+        const float f = pow2(exponent(other_m, all, c));
+        outside = lane < shares ? other_outside * f : 0.0f;
+        top_sum = lane < shares ? other_top * f : 0.0f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            outside += __shfl_xor_sync(kFull, outside, o);
+            top_sum += __shfl_xor_sync(kFull, top_sum, o);
         }
-        outside = joined;
+        outside = __shfl_sync(kFull, outside, 0);
+        top_sum = __shfl_sync(kFull, top_sum, 0);
         cluster.barrier_arrive();  // the shares' memory is read
-        top_sum *= pow2(exponent(m, all, c));
         cross += held * ((all - m) * a.inv_t);
         m = all;
         R = __fmul_rn(m, c);
@@ -468,25 +481,20 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     __syncthreads();
     // The top's own, over them.
     if (leads && !empty) {
-        const uint32_t j = static_cast<uint32_t>(id);
-        const bool scalar = j < w.head || j >= w.tail();
-        const uint32_t v = scalar ? 0 : (j - w.head) / kVec;
-        if (scalar ? share == 0 : v >= from && v < to) {
-            float taught_q = q;
-            if (!alone) {
-                taught_q = 0.0f;
-                for (uint32_t x = 0; x < a.t.top; ++x)
-                    if (s.id[x] == id) taught_q += s.q[x] * q_scale;
-            }
-            const float e = term(zt), p_j = e * k.inv_s;
-            put<T>(a, out + j, first + j, k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p_j * (1.0f - p_j), true, most);
+        float taught_q = q;
+        if (!alone) {
+            taught_q = 0.0f;
+            for (uint32_t x = 0; x < a.t.top; ++x)
+                if (s.id[x] == id) taught_q += s.q[x] * q_scale;
         }
+        const float e = term(zt), p_j = e * k.inv_s;
+        put<T>(a, out + id, first + id, k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p_j * (1.0f - p_j), true, most);
     }
     if constexpr (kCluster) cg::this_cluster().barrier_wait();
 }
 
 template <class T, int kVec, int kThreads, bool kCluster>
-__global__ void __launch_bounds__(kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares, uint32_t slots) {
+__global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares, uint32_t slots) {
     if (a.stopped != nullptr && *a.stopped) return;
     extern __shared__ __align__(16) unsigned char held[];
     __shared__ Shared<kThreads> s;

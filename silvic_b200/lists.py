@@ -52,11 +52,33 @@ class Distilled:
     hessian: Any = None
 
 
-def _type_of(tensor, what: str) -> int:
-    import torch
+# torch's part of this module, looked up by the first call: the package itself does without torch.
+_torch = None
+_TYPES: dict = {}
 
-    code = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}.get(
-        getattr(tensor, "dtype", None))
+
+def _use_torch():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _TYPES.update({torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16})
+        _torch = torch
+    return _torch
+
+
+def torch_float32():
+    return _use_torch().float32
+
+
+def stream(device: int) -> int:
+    """torch's current stream of a device, as a cudaStream_t."""
+    return _torch._C._cuda_getCurrentRawStream(device)
+
+
+def _type_of(tensor, what: str) -> int:
+    _use_torch()
+    code = _TYPES.get(getattr(tensor, "dtype", None))
     if code is None:
         raise ValueError(f"{what}: a float32, bfloat16 or float16 tensor")
     return code
@@ -65,22 +87,25 @@ def _type_of(tensor, what: str) -> int:
 def _row_stride(tensor, what: str) -> int:
     """Entries from one row of a 2-D tensor to the next; its rows are contiguous and lie apart."""
     rows, cols = tensor.shape
-    if cols > 1 and tensor.stride(1) != 1:
+    step, one = tensor.stride()
+    if cols > 1 and one != 1:
         raise ValueError(f"{what}: rows of contiguous entries")
-    if rows > 1 and tensor.stride(0) < cols:
+    if rows <= 1:
+        return cols
+    if step < cols:
         raise ValueError(f"{what}: rows that do not overlap")
-    return tensor.stride(0) if rows > 1 else cols
+    return step
 
 
 def lists_arg(scores, boundaries) -> _abi.Lists:
     """The lists of a 2-D tensor's rows, or of a 1-D tensor cut at `boundaries`."""
-    import torch
-
     code = _type_of(scores, "scores")
     if boundaries is None:
         if scores.dim() != 2:
             raise ValueError("scores: a 2-D tensor, or a 1-D one with boundaries")
-        return _abi.Lists(scores.data_ptr(), code, scores.shape[0], scores.shape[1], _row_stride(scores, "scores"), None)
+        rows, cols = scores.shape
+        return _abi.Lists(scores.data_ptr(), code, rows, cols, _row_stride(scores, "scores"), None)
+    torch = _torch
     if scores.dim() != 1 or (scores.shape[0] > 1 and scores.stride(0) != 1):
         raise ValueError("scores: a contiguous 1-D tensor with boundaries")
     if boundaries.dim() != 1 or boundaries.shape[0] < 1 or boundaries.dtype not in (torch.int32, torch.uint32) \
@@ -89,11 +114,44 @@ def lists_arg(scores, boundaries) -> _abi.Lists:
     return _abi.Lists(scores.data_ptr(), code, boundaries.shape[0] - 1, scores.shape[0], 0, boundaries.data_ptr())
 
 
+class Outputs:
+    """f32 and int32 outputs of `columns` values a list each, in one allocation beside the scores: a call's host time
+    is a few microseconds, and an allocation is the largest part of it."""
+
+    def __init__(self, scores, rows: int, columns):
+        self._rows, self._columns, self._starts = rows, columns, []
+        total = 0
+        for c in columns:
+            self._starts.append(total)
+            total += rows * c
+        self._buffer = scores.new_empty(total, dtype=_torch.float32)
+        base = self._buffer.data_ptr()
+        self.pointers = [base + 4 * s if rows * c else None for s, c in zip(self._starts, columns)]
+
+    def part(self, i: int):
+        c = self._columns[i]
+        return self._buffer.as_strided((self._rows, c), (c, 1), self._starts[i])
+
+    def flat(self, i: int):
+        return self._buffer.as_strided((self._rows,), (1,), self._starts[i])
+
+    def ids(self, i: int):
+        c = self._columns[i]
+        return self._buffer.view(_torch.int32).as_strided((self._rows, c), (c, 1), self._starts[i])
+
+
+def like(scores, rows: int, width: int, stride: int):
+    """Memory for derivatives of `scores`: rows `stride` entries apart, or (1-D scores) a flat copy of it."""
+    if scores.dim() == 1:
+        return scores.new_empty(scores.shape[0])
+    if stride == width:
+        return scores.new_empty((rows, width))
+    return scores.new_empty((rows, stride)).as_strided((rows, width), (stride, 1))
+
+
 def given_arg(given, num_lists: int):
     """The given entries as a contiguous int32 [lists, n] tensor (a 1-D one: an entry a list)."""
-    import torch
-
-    if given.dtype != torch.int32:
+    if given.dtype != _use_torch().int32:
         raise ValueError("given: an int32 tensor")
     if given.dim() == 1:
         given = given[:, None]
@@ -104,20 +162,16 @@ def given_arg(given, num_lists: int):
 
 def per_list_arg(values, num_lists: int, what: str):
     """An f32 value a list, contiguous."""
-    import torch
-
-    if values.dtype != torch.float32 or values.dim() != 1 or values.shape[0] != num_lists:
+    if values.dtype != _use_torch().float32 or values.dim() != 1 or values.shape[0] != num_lists:
         raise ValueError(f"{what}: a float32 tensor of {num_lists} values")
     return values.contiguous()
 
 
 def teacher_arg(teacher: TeacherTop, num_lists: int):
     """(the C struct, the tensors it points to) of a teacher's CUDA tensors."""
-    import torch
-
     ids, logits = teacher.ids, teacher.logits
     code = _type_of(logits, "the teacher's logits")
-    if ids.dtype != torch.int32 or ids.dim() != 2:
+    if ids.dtype != _torch.int32 or ids.dim() != 2:
         raise ValueError("the teacher's ids: a 2-D int32 tensor")
     if ids.shape[0] != num_lists or ids.shape != logits.shape:
         raise ValueError(f"a teacher of ids {tuple(ids.shape)} and logits {tuple(logits.shape)} for {num_lists} lists")
@@ -136,7 +190,7 @@ def teacher_arg(teacher: TeacherTop, num_lists: int):
 def check_device(device: int, tensors):
     """Every tensor on the handle's device; last among the checks."""
     for t in tensors:
-        if not t.is_cuda or t.device.index != device:
+        if t is not None and (not t.is_cuda or t.get_device() != device):
             raise ValueError(f"a tensor on {t.device}, not on the handle's device cuda:{device}")
 
 
