@@ -17,7 +17,6 @@
 // starts. A dense list too long for shared memory (or of scores so far from 0 that fma(z, c, -m c) loses its last bits) is read again for each
 // pass.
 #include <algorithm>
-#include <cfloat>
 
 #include "lists_device.cuh"
 
@@ -31,18 +30,18 @@ constexpr uint32_t kWarpEntries = 512;
 constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
 constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
-constexpr float kFar = 1048576.0f;   // |m c| from which an exponent is taken from the distance z - m
 
 constexpr uint32_t kBits = 65536;    // marks of a share: entries past so many share them
 
 // What a CTA keeps of its share of a list beside the scores.
 template <int kThreads>
 struct Shared {
-    float warp[6][kThreads / 32];
+    float warp[7][kThreads / 32];
     float m, outside, top;           // the share's reference and sums (with the rest: outside the top, and in it)
     __align__(16) int32_t id[kMaxTop];
     float q[kMaxTop];
     uint32_t again;                  // some entry's mark was set before
+    int32_t far;                     // far scores in the share
     uint32_t edge_bits;              // marks of the scalars outside the vectors
 };
 
@@ -156,6 +155,64 @@ __device__ __forceinline__ Slopes slopes_of(float w, float inv_t, float held, fl
     return k;
 }
 
+// Marks the teacher's entry `id` where it lies in this share (true). s.again: a mark that was set before.
+template <class T, int kVec, int kThreads>
+__device__ __forceinline__ bool mark_entry(Shared<kThreads>& s, uint32_t* bits, bool room, const Walk<T, kVec>& w, uint32_t from,
+                                           uint32_t to, uint32_t share, int32_t id) {
+    if (id < 0) return false;
+    const uint32_t j = static_cast<uint32_t>(id);
+    uint32_t before, mark;
+    if (j < w.head || j >= w.tail()) {
+        if (share != 0) return false;
+        mark = 1u << (j < w.head ? j : w.head + (j - w.tail()));
+        before = atomicOr(&s.edge_bits, mark);
+    } else {
+        if ((j - w.head) / kVec < from || (j - w.head) / kVec >= to) return false;
+        const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
+        mark = 1u << (bit & 31);
+        before = room ? atomicOr(&bits[bit / 32], mark) : mark;
+    }
+    if ((before & mark) != 0) s.again = 1;  // an index named twice, or one that shares its mark
+    return true;
+}
+
+// Whether entry `t` of the teacher is the first that names its index, and the only one (s.id is -1 up to the next
+// multiple of 4).
+template <int kThreads>
+__device__ __forceinline__ void lead(const Shared<kThreads>& s, int32_t id, uint32_t t, uint32_t top, bool& leads, bool& alone) {
+    uint32_t same = 0, before = 0;
+    for (uint32_t k = 0; k < top; k += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(&s.id[k]);
+        const uint32_t hit = (o.x == id ? 1u : 0u) | (o.y == id ? 2u : 0u) | (o.z == id ? 4u : 0u) | (o.w == id ? 8u : 0u);
+        if (hit != 0) {
+            same += __popc(hit);
+            before += __popc(k > t ? 0u : hit & ((1u << (t - k < 4 ? t - k : 4)) - 1u));
+        }
+    }
+    alone = same == 1;
+    leads = leads && before == 0;
+}
+
+// Marks of vector `v`'s entries, the share's first vector `from`. Where the marks are shared or there are none, the ids
+// themselves decide.
+template <class T, int kVec, int kThreads>
+__device__ __forceinline__ uint32_t marks_of(const Shared<kThreads>& s, const uint32_t* bits, bool room, const Walk<T, kVec>& w,
+                                             uint32_t from, uint32_t to, uint32_t top, uint32_t v) {
+    uint32_t m = ~0u;
+    if (room) {
+        const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
+        m = (bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
+    }
+    if (m != 0 && (!room || (to - from) * kVec > kBits)) {
+        m = 0;
+        for (uint32_t k = 0; k < top; ++k) {
+            const uint32_t e = static_cast<uint32_t>(s.id[k]) - w.at(v);
+            if (e < kVec) m |= 1u << e;
+        }
+    }
+    return m;
+}
+
 // One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). `data` holds `slots` vectors
 // (scores, for kVec 1), then the marks: where the share is no longer, it stays there.
 template <class T, int kVec, int kThreads, bool kCluster>
@@ -195,22 +252,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
     if (t == 0) s.edge_bits = s.again = 0;
     __syncthreads();
-    bool mine = false;  // the entry lies in this share
-    if (id >= 0) {
-        const uint32_t j = static_cast<uint32_t>(id);
-        uint32_t before = 0, mark = 0;
-        if (j < w.head || j >= w.tail()) {
-            mine = share == 0;
-            mark = 1u << (j < w.head ? j : w.head + (j - w.tail()));
-            before = atomicOr(&s.edge_bits, mark);
-        } else if ((j - w.head) / kVec >= from && (j - w.head) / kVec < to) {
-            mine = true;
-            const uint32_t bit = (j - w.head - from * kVec) & (kBits - 1);
-            mark = 1u << (bit & 31);
-            before = held_here ? atomicOr(&bits[bit / 32], mark) : mark;
-        }
-        if ((before & mark) != 0) s.again = 1;  // an index named twice, or one that shares its mark
-    }
+    const bool mine = mark_entry(s, bits, held_here, w, from, to, share, id);
     // Vector `v` of the share; a run between boundaries, entry by entry, is read from its place each time.
     auto get = [&](uint32_t v, float(&x)[kVec]) {
         if constexpr (kVec == 1)
@@ -218,22 +260,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         else
             data[v].values(x);
     };
-    // Marks of vector `v`'s entries. Where the marks are shared or there are none, the ids themselves decide.
-    auto marked = [&](uint32_t v) {
-        uint32_t m = ~0u;
-        if (held_here) {
-            const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
-            m = (bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
-        }
-        if (m != 0 && (!held_here || (to - from) * kVec > kBits)) {
-            m = 0;
-            for (uint32_t k = 0; k < a.t.top; ++k) {
-                const uint32_t e = static_cast<uint32_t>(s.id[k]) - w.at(v);
-                if (e < kVec) m |= 1u << e;
-            }
-        }
-        return m;
-    };
+    auto marked = [&](uint32_t v) { return marks_of(s, bits, held_here, w, from, to, a.t.top, v); };
     // The maxima of the scores and of the teacher's.
     float m = fmaxf(edge, zt);  // with the top's scores, so that no share's reference lies far below them
     if constexpr (kVec == 1) {
@@ -315,19 +342,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     const bool edge_marked = edge_at < n && ((s.edge_bits >> t) & 1u) != 0;
     if (edge_at < n && !(rest && edge_marked)) sum += term(edge);
     bool leads = mine, alone = true;  // the first of the teacher's entries that names this index, and the only one
-    if (s.again != 0 && t < a.t.top) {
-        uint32_t same = 0, before = 0;
-        for (uint32_t k = 0; k < a.t.top; k += 4) {  // (s.id is -1 up to the next multiple of 4)
-            const int4 o = *reinterpret_cast<const int4*>(&s.id[k]);
-            const uint32_t hit = (o.x == id ? 1u : 0u) | (o.y == id ? 2u : 0u) | (o.z == id ? 4u : 0u) | (o.w == id ? 8u : 0u);
-            if (hit != 0) {
-                same += __popc(hit);
-                before += __popc(k > t ? 0u : hit & ((1u << (t - k < 4 ? t - k : 4)) - 1u));
-            }
-        }
-        alone = same == 1;
-        leads = leads && before == 0;
-    }
+    if (s.again != 0 && t < a.t.top) lead(s, id, t, a.t.top, leads, alone);
     // The teacher's terms, not yet divided by their sum where the top is all of it.
     const float base = rest ? a.t.log_sum[i] : y_max;
     float q = id >= 0 ? expf(y - base) : 0.0f;
@@ -493,6 +508,173 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     if constexpr (kCluster) cg::this_cluster().barrier_wait();
 }
 
+// The loss alone of one dense list: its sums are taken while it is read, about the maximum of the first batch (moved
+// where later entries lie far above it). False: far scores, which distill_list() takes.
+template <class T, int kVec, int kThreads, bool kCluster>
+__device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, const DistillArgs& a, uint32_t i, uint32_t share,
+                                          uint32_t shares) {
+    constexpr int kBatch = 4;  // vectors a thread has in flight
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    uint64_t first;
+    uint32_t n;
+    list_range(a.l, i, first, n);
+    const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
+    uint32_t from = 0, to = w.vectors;
+    if constexpr (kCluster) {
+        const uint32_t shift = __ffs(shares) - 1;
+        from = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * share) >> shift);
+        to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
+    }
+    const float c = __fmul_rn(kLog2E, a.inv_t);
+    const bool rest = a.t.log_sum != nullptr;
+    Pack<T, kVec> p[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const uint32_t v = from + u * kThreads + t;
+        if (v < to)
+            p[u].load(w.z + w.at(v));
+        else
+            p[u].masked();
+    }
+    const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
+    float edge[1] = {edge_at < n ? to_float(w.z[edge_at]) : -CUDART_INF_F};
+    int32_t id = -1;
+    float y = -CUDART_INF_F, zt = -CUDART_INF_F;
+    if (t < a.t.top) {
+        teacher_entry(a, i, t, n, id, y);
+        if (id >= 0) zt = to_float(w.z[id]);
+    }
+    bool mine = false;
+    if (rest) {  // the top's entries, which the sum leaves out
+        if (t < kMaxTop) s.id[t] = id;
+        const uint32_t words = (min(kBits, (to - from) * kVec) + 31) / 32;
+        for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
+        if (t == 0) s.edge_bits = s.again = 0;
+        __syncthreads();
+        mine = mark_entry(s, bits, true, w, from, to, share, id);
+    }
+    Pack<T, kVec> top = p[0];
+#pragma unroll
+    for (int u = 1; u < kBatch; ++u) top.raise(p[u]);
+    float m = fmaxf(edge[0], zt), x[kVec];
+    top.values(x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) m = fmaxf(m, x[e]);
+    m = warp_max(m);
+    float y_max = warp_max(y);
+    if (lane == 0) {
+        s.warp[0][warp] = m;
+        s.warp[1][warp] = y_max;
+    }
+    const bool taught = __syncthreads_or(id >= 0) != 0;
+    m = max_of<kThreads>(s.warp[0]);
+    y_max = fmaxf(max_of<kThreads>(s.warp[1]), -FLT_MAX);
+    Reader<false> r(m, c);
+    auto read = [&](bool look) {
+        for (uint32_t base = from; base < to; base += kBatch * kThreads) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const uint32_t v = base + u * kThreads + t;
+                if (v < to) {
+                    p[u].values(x);
+                    const uint32_t next = v + kBatch * kThreads;
+                    if (next < to) p[u].load(w.z + w.at(next));
+                    const uint32_t skip = look ? marks_of(s, bits, true, w, from, to, a.t.top, v) : 0;
+                    if (skip != 0) {
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e)
+                            if ((skip >> e) & 1u) x[e] = -CUDART_INF_F;
+                    }
+                    r.add(x);
+                }
+            }
+        }
+    };
+    if (rest)
+        read(true);
+    else
+        read(false);
+    if (edge_at < n && !(rest && ((s.edge_bits >> t) & 1u) != 0)) r.add(edge);
+    // The teacher's terms about the first reference, the sums about the largest.
+    m = fmaxf(m, -FLT_MAX);
+    const float base = rest ? a.t.log_sum[i] : y_max;
+    Stats mine_sum = settled(r.x, c);
+    const float warp_m = warp_max(mine_sum.m);
+    rebase(mine_sum, warp_m, c);
+    const float sum_part = warp_sum(mine_sum.s);
+    if (warp * 32 < a.t.top) {
+        bool leads = mine, alone = true;
+        if (rest && s.again != 0 && t < a.t.top) lead(s, id, t, a.t.top, leads, alone);
+        const float q = id >= 0 ? expf(y - base) : 0.0f;
+        const float top_part = warp_sum(rest && leads ? pow2(exponent(zt, m, c)) : 0.0f);
+        const float held_part = warp_sum(q);
+        const float cross_part = warp_sum(q != 0.0f ? q * (y - base - (zt - m) * a.inv_t) : 0.0f);
+        if (lane == 0) {
+            s.warp[3][warp] = top_part;
+            s.warp[4][warp] = held_part;
+            s.warp[5][warp] = cross_part;
+        }
+    } else if (lane == 0) {
+        s.warp[3][warp] = s.warp[4][warp] = s.warp[5][warp] = 0.0f;
+    }
+    if (lane == 0) {
+        s.warp[6][warp] = warp_m;
+        s.warp[2][warp] = sum_part;
+    }
+    bool far = __syncthreads_or(r.far()) != 0;
+    float all = fmaxf(max_of<kThreads>(s.warp[6]), m);
+    const uint32_t k = lane & (kThreads / 32 - 1);
+    float outside = lane < kThreads / 32 ? s.warp[2][k] * pow2(exponent(s.warp[6][k], all, c)) : 0.0f;
+    outside = warp_sum(outside);
+    float top_sum = sum_of<kThreads>(s.warp[3]) * pow2(exponent(m, all, c));
+    float held = sum_of<kThreads>(s.warp[4]);
+    float cross = sum_of<kThreads>(s.warp[5]);
+    if constexpr (kCluster) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (t == 0) {
+            s.m = all;
+            s.outside = outside;
+            s.top = top_sum;
+            s.far = far;
+        }
+        cluster.sync();
+        const auto* other = cluster.map_shared_rank(&s, lane & (shares - 1));
+        const float other_m = other->m, other_outside = other->outside, other_top = other->top;
+        far = __any_sync(kFull, other->far);
+        all = warp_max(other_m);
+        const float f = pow2(exponent(other_m, all, c));
+        outside = warp_sum(lane < shares ? other_outside * f : 0.0f);
+        top_sum = warp_sum(lane < shares ? other_top * f : 0.0f);
+        cluster.sync();  // the shares' memory is read
+    }
+    if (far) return false;
+    if (t == 0 && share == 0) {
+        cross += held * ((all - m) * a.inv_t);
+        if (!rest && held != 0.0f) {
+            cross = cross / held - logf(held);
+            held = 1.0f;
+        }
+        const float sum = outside + top_sum;
+        const float rest_q = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+        const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
+        a.loss[i] = sum == 0.0f || !taught ? 0.0f : weight * loss_of(cross, held, sum, outside, rest_q);
+    }
+    return true;
+}
+
+template <class T, int kVec, int kThreads, bool kCluster>
+__global__ void __launch_bounds__(kThreads) distill_loss_kernel(DistillArgs a, uint32_t shares) {
+    __shared__ Shared<kThreads> s;
+    extern __shared__ __align__(16) unsigned char held[];
+    uint32_t* bits = reinterpret_cast<uint32_t*>(held);
+    const uint32_t shift = kCluster ? __ffs(shares) - 1 : 0;
+    const uint32_t i = blockIdx.x >> shift, share = blockIdx.x & (shares - 1);
+    if (loss_list<T, kVec, kThreads, kCluster>(s, bits, a, i, share, shares)) return;
+    __syncthreads();
+    Maxima most;
+    distill_list<T, kVec, kThreads, kCluster>(s, nullptr, 0, bits, a, i, share, shares, most);
+}
+
 template <class T, int kVec, int kThreads, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares, uint32_t slots) {
     if (a.stopped != nullptr && *a.stopped) return;
@@ -515,7 +697,8 @@ struct WarpShared {
 
 // A list of at most 32 kItems entries by one warp, in registers; kTop of the teacher's entries a lane.
 template <class T, int kItems, int kTop>
-__device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n, Maxima& most) {
+__device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n,
+                                             const int32_t (&ids)[kTop], const float (&logits)[kTop], Maxima& most) {
     const uint32_t lane = threadIdx.x & 31;
     const T* z = static_cast<const T*>(a.l.scores) + first;
     const float c = __fmul_rn(kLog2E, a.inv_t);
@@ -538,10 +721,11 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         y[u] = zt[u] = -CUDART_INF_F;
         const uint32_t k = u * 32 + lane;
         if (k < a.t.top) {
-            teacher_entry(a, i, k, n, id[u], y[u]);
+            if (ids[u] >= 0 && static_cast<uint32_t>(ids[u]) < n) id[u] = ids[u];
             s.id[k] = id[u];
         }
         if (id[u] >= 0) {
+            y[u] = logits[u] * a.inv_t;
             zt[u] = to_float(z[id[u]]);
             atomicOr(&s.bits[id[u] / 32], 1u << (id[u] & 31));
             taught = true;
@@ -636,7 +820,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
 
 // A warp per list; a longer one among them by the whole CTA.
 template <class T, int kTop>
-__global__ void __launch_bounds__(kWarpThreads) distill_warps_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillArgs a) {
     if (a.stopped != nullptr && *a.stopped) return;
     constexpr uint32_t kLists = kWarpThreads / 32;
     __shared__ WarpShared warps[kLists];
@@ -647,14 +831,24 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warps_kernel(DistillArgs
     uint32_t n = 0;
     Maxima most;
     if (i < a.l.lists) {
+        // The teacher's entries, on their way beside the boundaries.
+        int32_t ids[kTop];
+        float logits[kTop];
+#pragma unroll
+        for (int u = 0; u < kTop; ++u) {
+            const uint32_t k = u * 32 + (threadIdx.x & 31);
+            const uint64_t at = static_cast<uint64_t>(i) * a.t.stride + k;
+            ids[u] = k < a.t.top ? a.t.ids[at] : -1;
+            logits[u] = k < a.t.top ? load_typed(a.t.logits, a.t.type, at) : 0.0f;
+        }
         list_range(a.l, i, first, n);
         WarpShared& s = warps[threadIdx.x >> 5];
         if (n <= 128)
-            distill_warp<T, 4, kTop>(s, a, i, first, n, most);
+            distill_warp<T, 4, kTop>(s, a, i, first, n, ids, logits, most);
         else if (n <= 256)
-            distill_warp<T, 8, kTop>(s, a, i, first, n, most);
+            distill_warp<T, 8, kTop>(s, a, i, first, n, ids, logits, most);
         else if (n <= kWarpEntries)
-            distill_warp<T, 16, kTop>(s, a, i, first, n, most);
+            distill_warp<T, 16, kTop>(s, a, i, first, n, ids, logits, most);
     }
     if (__syncthreads_or(n > kWarpEntries) != 0)
         for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
@@ -674,12 +868,13 @@ size_t rows_smem(uint32_t slots) {
     return ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)) + (std::min<size_t>(entries, kBits) + 31) / 32 * 4;
 }
 
-template <class T, int kVec, int kThreads>
-void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStream_t s) {
+// A launch of `shares` CTAs a list, as clusters where that is more than one.
+template <class Kernel, class... Args>
+void launch_shares(Kernel* kernel, const DistillArgs& a, int threads, size_t smem, uint32_t shares, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(a.l.lists * shares);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = rows_smem<T, kVec>(slots);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
     config.stream = s;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -687,9 +882,21 @@ void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStre
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = shares > 1 ? 1 : 0;
-    auto* kernel = shares > 1 ? distill_rows_kernel<T, kVec, kThreads, true> : distill_rows_kernel<T, kVec, kThreads, false>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHeld) != cudaSuccess) return;
-    cudaLaunchKernelEx(&config, kernel, a, shares, slots);
+    // (48 KB go without the attribute; setting it is host time)
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHeld) != cudaSuccess) return;
+    cudaLaunchKernelEx(&config, kernel, a, shares, args...);
+}
+
+template <class T, int kVec, int kThreads>
+void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStream_t s) {
+    launch_shares(shares > 1 ? distill_rows_kernel<T, kVec, kThreads, true> : distill_rows_kernel<T, kVec, kThreads, false>, a,
+                  kThreads, rows_smem<T, kVec>(slots), shares, s, slots);
+}
+
+template <class T, int kVec, int kThreads>
+void launch_loss(const DistillArgs& a, uint32_t shares, uint64_t entries, cudaStream_t s) {
+    launch_shares(shares > 1 ? distill_loss_kernel<T, kVec, kThreads, true> : distill_loss_kernel<T, kVec, kThreads, false>, a,
+                  kThreads, static_cast<size_t>(std::min<uint64_t>(entries / shares + kVec, kBits) / 32 + 1) * 4, shares, s);
 }
 
 template <class T>
@@ -710,6 +917,14 @@ void launch_typed(const DistillArgs& a, cudaStream_t s) {
             launch_rows<T, 1, 128>(a, shares, 0, s);
         else
             launch_rows<T, 1, 256>(a, shares, 0, s);
+        return;
+    }
+    if (a.grad == nullptr && a.hess == nullptr) {
+        if (a.loss == nullptr) return;
+        if (mean / shares <= 4096)
+            launch_loss<T, kVec, 128>(a, shares, mean, s);
+        else
+            launch_loss<T, kVec, 256>(a, shares, mean, s);
         return;
     }
     // As many shares as hold the list in kHeld bytes each, else in kMaxHeld (longer: read again).

@@ -1,6 +1,8 @@
 // lists_device.cuh — what the kernels over lists of candidates share on the device.
 #pragma once
 
+#include <cfloat>
+
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -177,6 +179,92 @@ struct Pack<T, 1> {
     __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = to_float(raw); }
     __device__ __forceinline__ void raise(const Pack& o) { raw = to_float(o.raw) > to_float(raw) || raw != raw ? o.raw : raw; }
     __device__ __forceinline__ void masked() { raw = from_float<T>(-CUDART_INF_F); }
+};
+
+// A softmax's statistics: the reference m, S = sum 2^y and V = sum 2^y y about it, y = (z - m) log2(e) / T.
+struct Stats {
+    float m, s, v;
+};
+
+// Statistics about another reference.
+__device__ __forceinline__ void rebase(Stats& a, float m, float c) {
+    const float y = exponent(a.m, m, c), f = pow2(y);
+    a.v = f * (a.v + a.s * y);
+    a.s *= f;
+    a.m = m;
+}
+
+// Statistics about R = m c rounded, so that an exponent is one fma(z, c, -R).
+struct Rounded {
+    Stats a;  // a.m the reference, a.s and a.v about r
+    float r;
+};
+
+// The statistics about m itself: the rounding of R is put back.
+__device__ __forceinline__ Stats settled(const Rounded& x, float c) {
+    if (x.a.s == 0.0f) return {x.a.m, 0.0f, 0.0f};
+    const float y = -__fmaf_rn(x.a.m, c, -x.r), f = pow2(y);
+    return {x.a.m, x.a.s * f, f * __fmaf_rn(x.a.s, y, x.a.v)};
+}
+
+// The statistics about a higher reference.
+static __device__ __noinline__ Rounded moved(Rounded x, float m, float c) {
+    Stats now = settled(x, c);
+    rebase(now, m, c);
+    const float r = __fmul_rn(m, c);
+    const float y = __fmaf_rn(m, c, -r), f = pow2(y);
+    return {{m, now.s * f, f * __fmaf_rn(now.s, y, now.v)}, r};
+}
+
+constexpr float kSlack = 4.0f;        // log2 units that an entry may lie above the reference before it moves
+constexpr float kFar = 1048576.0f;    // |R| from which its rounding matters: exponents are then taken from z - m
+
+// One thread's running statistics; kParts: V too.
+template <bool kParts>
+struct Reader {
+    Rounded x;
+    float c, limit;
+
+    // About the maximum of the first entries (-inf: about the first unmasked entry that comes).
+    __device__ __forceinline__ Reader(float m, float scale) : c(scale), limit(m + kSlack / scale) {
+        x.a = {fmaxf(m, -FLT_MAX), 0.0f, 0.0f};
+        x.r = m == -CUDART_INF_F ? 0.0f : __fmul_rn(m, scale);
+    }
+    __device__ __forceinline__ bool far() const { return !(fabsf(x.r) < kFar); }
+    // Adds entries; their maximum.
+    template <int kCount>
+    __device__ __forceinline__ float add(const float (&z)[kCount]) {
+        float most = z[0];
+#pragma unroll
+        for (int e = 1; e < kCount; ++e) most = fmaxf(most, z[e]);
+        if (most > limit) {
+            x = moved(x, most, c);
+            limit = most + kSlack / c;
+        }
+        if constexpr (kCount == 1) {
+            const float y = max_nan(__fmaf_rn(z[0], c, -x.r), -200.0f), p = pow2(y);
+            x.a.s += p;
+            if (kParts) x.a.v = __fmaf_rn(p, y, x.a.v);
+        } else {
+            // pairs in one instruction: issue bounds the kernel before memory
+            const float2 cc = make_float2(c, c), minus_r = make_float2(-x.r, -x.r);
+            float2 sum = make_float2(0.0f, 0.0f), part = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int e = 0; e < kCount; e += 2) {
+                float2 y = __ffma2_rn(make_float2(z[e], z[e + 1]), cc, minus_r);
+                if (kParts) {  // a masked entry's 0 times its exponent is 0
+                    y.x = max_nan(y.x, -200.0f);
+                    y.y = max_nan(y.y, -200.0f);
+                }
+                const float2 p = make_float2(pow2(y.x), pow2(y.y));
+                sum = __fadd2_rn(sum, p);
+                if (kParts) part = __ffma2_rn(p, y, part);
+            }
+            x.a.s += sum.x + sum.y;
+            if (kParts) x.a.v += part.x + part.y;
+        }
+        return most;
+    }
 };
 
 __device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -10,8 +10,6 @@
 // entries reach, and so a filter; entries that pass it are gathered in shared memory and ranked at the end. A list
 // whose order defeats the filter (more candidates than the buffer holds) has its alternatives selected again, digit by
 // digit of their keys.
-#include <cfloat>
-
 #include "lists_device.cuh"
 
 namespace cg = cooperative_groups;
@@ -25,19 +23,6 @@ constexpr int kWarpThreads = 256;        // the warp kernel's CTAs
 constexpr uint32_t kCandidates = 2048;   // keys that a CTA gathers
 constexpr int kBatch = 4;                // vectors a thread holds in flight
 constexpr uint32_t kSingle = 0x80000000u;
-constexpr float kSlack = 4.0f;           // log2 units that an entry may lie above the reference before it moves
-
-struct Stats {
-    float m, s, v;  // the reference, the sum of 2^y, the sum of 2^y y
-};
-
-// Statistics about another reference.
-__device__ __forceinline__ void rebase(Stats& a, float m, float c) {
-    const float y = exponent(a.m, m, c), f = pow2(y);
-    a.v = f * (a.v + a.s * y);
-    a.s *= f;
-    a.m = m;
-}
 
 // What a CTA keeps of its share of a list.
 template <int kThreads>
@@ -156,79 +141,6 @@ __device__ __forceinline__ uint32_t take(uint32_t* counter) {
     return at;
 }
 
-// Statistics about R = m c rounded, so that an exponent is one fma(z, c, -R).
-struct Rounded {
-    Stats a;  // a.m the reference, a.s and a.v about r
-    float r;
-};
-
-// The statistics about m itself: the rounding of R is put back.
-__device__ __forceinline__ Stats settled(const Rounded& x, float c) {
-    if (x.a.s == 0.0f) return {x.a.m, 0.0f, 0.0f};
-    const float y = -__fmaf_rn(x.a.m, c, -x.r), f = pow2(y);
-    return {x.a.m, x.a.s * f, f * __fmaf_rn(x.a.s, y, x.a.v)};
-}
-
-// The statistics about a higher reference.
-__device__ __noinline__ Rounded moved(Rounded x, float m, float c) {
-    Stats now = settled(x, c);
-    rebase(now, m, c);
-    const float r = __fmul_rn(m, c);
-    const float y = __fmaf_rn(m, c, -r), f = pow2(y);
-    return {{m, now.s * f, f * __fmaf_rn(now.s, y, now.v)}, r};
-}
-
-// One thread's running statistics and its filter for alternatives.
-template <class T, int kVec, int kThreads>
-struct Reader {
-    Shared<kThreads>& s;
-    Rounded x;
-    float c, limit, bound;
-
-    // About the maximum of the first entries (-inf: about the first unmasked entry that comes).
-    __device__ __forceinline__ Reader(Shared<kThreads>& shared, float m, float scale, float bound_)
-        : s(shared), c(scale), limit(m + kSlack / scale), bound(bound_) {
-        x.a = {fmaxf(m, -FLT_MAX), 0.0f, 0.0f};
-        x.r = m == -CUDART_INF_F ? 0.0f : __fmul_rn(m, scale);
-    }
-    // Whether R is so large that its rounding matters: far_stats() takes over.
-    __device__ __forceinline__ bool far() const { return !(fabsf(x.r) < 1048576.0f); }
-    template <int kCount>
-    __device__ __forceinline__ void add(const float (&z)[kCount], uint32_t first) {
-        float most = z[0];
-#pragma unroll
-        for (int e = 1; e < kCount; ++e) most = fmaxf(most, z[e]);
-        if (most > limit) {
-            x = moved(x, most, c);
-            limit = most + kSlack / c;
-        }
-        if constexpr (kCount == 1) {
-            const float y = max_nan(__fmaf_rn(z[0], c, -x.r), -200.0f), p = pow2(y);
-            x.a.s += p;
-            x.a.v = __fmaf_rn(p, y, x.a.v);
-        } else {
-            // pairs in one instruction: issue bounds the kernel before memory
-            const float2 cc = make_float2(c, c), minus_r = make_float2(-x.r, -x.r);
-            float2 sum = make_float2(0.0f, 0.0f), part = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int e = 0; e < kCount; e += 2) {
-                float2 y = __ffma2_rn(make_float2(z[e], z[e + 1]), cc, minus_r);
-                y.x = max_nan(y.x, -200.0f);  // a masked entry's 0 times its exponent is 0
-                y.y = max_nan(y.y, -200.0f);
-                const float2 p = make_float2(pow2(y.x), pow2(y.y));
-                sum = __fadd2_rn(sum, p);
-                part = __ffma2_rn(p, y, part);
-            }
-            x.a.s += sum.x + sum.y;
-            x.a.v += part.x + part.y;
-        }
-        if (most >= bound) {  // the vector (or the scalar) holds a candidate
-            const uint32_t at = take(&s.count);
-            if (at < kCandidates) s.held[at] = kCount == 1 ? first | kSingle : first;
-        }
-    }
-};
-
 // The statistics of a share of far scores (about 700,000 T and more from 0): the maximum first, then each entry's distance from it.
 template <class T, int kVec, int kThreads>
 __device__ __noinline__ Stats far_stats(Shared<kThreads>& s, const T* z, uint32_t n, uint32_t from, uint32_t to, bool edges,
@@ -332,10 +244,15 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     }
     __syncthreads();
     // Masked entries are no alternatives.
-    const float bound = a.top > 0 ? fmaxf(score_of(s.bound), -FLT_MAX) : CUDART_NAN_F;
+    float bound = a.top > 0 ? fmaxf(score_of(s.bound), -FLT_MAX) : CUDART_NAN_F;
     // One pass: the statistics about the first batch's maximum (moved where later entries lie far above it), and the
     // entries that reach the bound.
-    Reader<T, kVec, kThreads> r(s, most, c, bound);
+    Reader<true> r(most, c);
+    // A vector (or a scalar) that holds a candidate.
+    auto hold = [&](uint32_t first_entry) {
+        const uint32_t at = take(&s.count);
+        if (at < kCandidates) s.held[at] = first_entry;
+    };
     uint32_t batch = 0;
     for (uint32_t base = from; base < to; base += kBatch * kThreads) {
 #pragma unroll
@@ -346,24 +263,24 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
                 p[u].values(x);
                 const uint32_t next = v + kBatch * kThreads;
                 if (next < to) p[u].load(w.z + w.at(next));
-                r.add(x, w.at(v));
+                if (r.add(x) >= bound) hold(w.at(v));
             }
         }
         // Each time the part that is read has doubled: many candidates are cut to the alternatives so far, whose last
         // is the bound from here on. So candidates stay few however long the list is, unless its order defeats that.
         if ((++batch & (batch - 1)) == 0 && a.top > 0 && base + kBatch * kThreads < to) {
             __syncthreads();
-            if (s.count > max(64u, 2 * a.top) && expand<T, kVec, kThreads>(s, w.z, r.bound)) {
+            if (s.count > max(64u, 2 * a.top) && expand<T, kVec, kThreads>(s, w.z, bound)) {
                 rank_candidates(s, s.keys, a.top);
                 __syncthreads();
                 for (uint32_t k = t; k < a.top; k += kThreads) s.held[k] = index_of(s.best[k]) | kSingle;
-                r.bound = score_of(static_cast<uint32_t>(s.best[a.top - 1] >> 32));
+                bound = score_of(static_cast<uint32_t>(s.best[a.top - 1] >> 32));
                 if (t == 0) s.count = a.top;
             }
             __syncthreads();
         }
     }
-    if (edge_at < n) r.add(edge, edge_at);
+    if (edge_at < n && r.add(edge) >= bound) hold(edge_at | kSingle);
     // The share's statistics.
     Stats mine = settled(r.x, c);
     if (__syncthreads_or(r.far())) mine = far_stats<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, c);
@@ -388,7 +305,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     }
     // The share's alternatives.
     if (a.top > 0) {
-        if (!expand<T, kVec, kThreads>(s, w.z, r.bound))
+        if (!expand<T, kVec, kThreads>(s, w.z, bound))
             select_candidates<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, a.top);
         rank_candidates(s, s.keys, a.top);
     }
@@ -490,48 +407,60 @@ __device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i
         const float given = id >= 0 && static_cast<uint32_t>(id) < n ? to_float(z[id]) : -CUDART_INF_F;
         a.given_out[at] = given == -CUDART_INF_F ? given : (given - m) * a.inv_t - log_s;
     }
-    // The alternatives, one a round: each lane offers its best entry that is not taken (a bit each).
-    uint32_t taken = 0;
-    float out = -CUDART_INF_F;
-    int32_t out_id = -1;
-    uint32_t best = 0, best_k = 0;
-    auto offer = [&] {
-        best = 0;
+    // The alternatives, one a round: each lane keeps its entries in order and offers the first that is left.
+    if (a.top == 0) return;
+    unsigned long long key[kItems];
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            const uint32_t o = x[k] == -CUDART_INF_F || ((taken >> k) & 1u) != 0 ? 0u : order_of(x[k]);
-            if (o > best) {
-                best = o;
-                best_k = k;
+    for (int k = 0; k < kItems; ++k) key[k] = x[k] > -CUDART_INF_F || x[k] != x[k] ? order_key(x[k], k * 32 + lane) : 0ull;
+#pragma unroll
+    for (int size = 2; size <= kItems; size <<= 1)  // a bitonic network over the lane's own, largest first
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1)
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                const int o = k ^ stride;
+                if (o > k) {
+                    const bool swap = (key[k] < key[o]) == ((k & size) == 0);
+                    const unsigned long long u = swap ? key[o] : key[k], v = swap ? key[k] : key[o];
+                    key[k] = u;
+                    key[o] = v;
+                }
             }
-        }
-    };
-    if (a.top > 0) offer();
+    uint32_t out_order = 0, out_low = 0;
     for (uint32_t r = 0; r < a.top; ++r) {
-        const uint32_t most_o = __reduce_max_sync(kFull, best);
-        const uint32_t j = __reduce_min_sync(kFull, best == most_o ? best_k * 32 + lane : 0xFFFFFFFFu);
-        if (most_o != 0 && (r & 31) == lane) out_id = static_cast<int32_t>(j);
-        if (most_o != 0 && (j & 31) == lane) {
-            taken |= 1u << best_k;
-            offer();
+        const uint32_t order = static_cast<uint32_t>(key[0] >> 32), low = static_cast<uint32_t>(key[0]);
+        const uint32_t most_order = __reduce_max_sync(kFull, order);
+        uint32_t who = __ballot_sync(kFull, order == most_order);
+        if ((who & (who - 1)) != 0) {  // a tie: the lower index
+            const uint32_t most_low = __reduce_max_sync(kFull, order == most_order ? low : 0u);
+            who = __ballot_sync(kFull, order == most_order && low == most_low);
+        }
+        const uint32_t winner = __ffs(who) - 1;
+        const uint32_t won = __shfl_sync(kFull, low, winner);
+        if (lane == (r & 31)) {
+            out_order = most_order;
+            out_low = won;
+        }
+        if (lane == winner) {
+#pragma unroll
+            for (int k = 0; k + 1 < kItems; ++k) key[k] = key[k + 1];
+            key[kItems - 1] = 0;
         }
         if ((r & 31) == 31 || r + 1 == a.top) {  // 32 alternatives leave together
-            const uint32_t base = r & ~31u;
-            if (base + lane < a.top) {
-                const uint64_t at = static_cast<uint64_t>(i) * a.top + base + lane;
-                if (out_id >= 0) out = (to_float(z[out_id]) - m) * a.inv_t - log_s;
-                a.top_ids[at] = out_id;
-                a.top_out[at] = out;
+            const uint32_t at_top = (r & ~31u) + lane;
+            if (at_top < a.top) {
+                const uint64_t at = static_cast<uint64_t>(i) * a.top + at_top;
+                a.top_ids[at] = out_order == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - out_low);
+                a.top_out[at] = out_order == 0 ? -CUDART_INF_F : (score_of(out_order) - m) * a.inv_t - log_s;
             }
-            out = -CUDART_INF_F;
-            out_id = -1;
+            out_order = 0;
         }
     }
 }
 
 // A warp per list; a longer one among them by the whole CTA.
 template <class T>
-__global__ void __launch_bounds__(kWarpThreads) log_probs_warps_kernel(LogProbsArgs a) {
+__global__ void __launch_bounds__(kWarpThreads, 4) log_probs_warps_kernel(LogProbsArgs a) {
     __shared__ __align__(16) Shared<kWarpThreads> shared;
     constexpr uint32_t kLists = kWarpThreads / 32;
     const uint32_t base = blockIdx.x * kLists, i = base + (threadIdx.x >> 5);

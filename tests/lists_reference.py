@@ -152,7 +152,9 @@ def check_distill(z, ids, logits, t, log_sum, w, got: dict, step: float, least: 
         outside = ~teach(n, ids, logits, t, log_sum)[1]
         p = softmax(z, t)[0]
         rest_p = p[outside].sum()
-        tol = want["scale"] * (relative + 4 * U * x) + step * np.abs(want["grad"]) * 1.001 + least
+        # a term exp((z - m) / T) below 2^-126 is 0: p is off by 2^-126 (S >= 1), its multiples by as much of theirs
+        tiny = 2.0 ** -125 * abs(w) / t * (1 + held + (1 / rest_p if rest_p > 0 else 0.0))
+        tol = want["scale"] * (relative + 4 * U * x) + step * np.abs(want["grad"]) * 1.001 + least + tiny
         if rest_p > 0:
             tol = tol + np.where(outside, abs(w) / t * p / rest_p * rest_slack, 0.0) + abs(w) / t * p * rest_slack
         bad = ~(np.abs(got["grad"] - want["grad"]) <= tol)
@@ -161,6 +163,6 @@ def check_distill(z, ids, logits, t, log_sum, w, got: dict, step: float, least: 
         p = softmax(z, t)[0]
         # 1 - p is off by p (2 slack + 3 U x) + U, whatever it is itself
         tol = (want["hess"] + abs(w) / t ** 2 * p * p) * (relative + 4 * U * x) + abs(w) / t ** 2 * p * (rest_slack + 4 * U)
-        tol = tol + step * np.abs(want["hess"]) * 1.001 + least
+        tol = tol + step * np.abs(want["hess"]) * 1.001 + least + 2.0 ** -125 * abs(w) / t ** 2 * (1 + held)
         bad = ~(np.abs(got["hess"] - want["hess"]) <= tol)
         assert not bad.any(), (np.nonzero(bad)[0][:5], got["hess"][bad][:5], want["hess"][bad][:5], tol[bad][:5])

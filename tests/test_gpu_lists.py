@@ -606,3 +606,31 @@ def test_log_probs_of_far_scores(backend, type_, lists, width):
         got = backend.log_probs(scores, given=torch.from_numpy(ids).cuda(), top=9, temperature=t)
         check_log_probs(scores[:12], rows_of(scores[:12]), ids, 9, t,
                         type(got)(*[v[:12] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("lists,width", [(3, 5000), (300, 20011)])
+def test_distill_of_far_scores(backend, lists, width, type_, rest):
+    """The lists of test_log_probs_of_far_scores, the loss alone and with its gradients."""
+    rng = np.random.RandomState(width)
+    z = rng.randn(lists, width) * 3
+    z[0] = -1.0e30
+    z[0, ::7] *= 1.0 + 2.0 ** -7
+    z[1] += 4.0e6
+    z[2, : width - 50] = -np.inf
+    if lists > 3:
+        z[3] += np.linspace(-300, 300, width)
+        z[4, : width - 40] = -np.inf
+        z[4, width - 40:] = torch.finfo(TYPES[type_]).min
+        z[5, : width - 40] = -1.0e5
+    scores = torch.from_numpy(z).to(TYPES[type_]).cuda()
+    ids = np.stack([width - 1 - rng.choice(40, 6, replace=False) for _ in range(lists)]).astype(np.int32)
+    logits = rng.randn(lists, 6) * 2
+    logits = torch.from_numpy(logits).float().cuda()
+    log_sum = torch.logsumexp(logits.double(), 1).float() + 0.3 if rest else None
+    teacher = TeacherTop(torch.from_numpy(ids).cuda(), logits, log_sum)
+    some = TeacherTop(teacher.ids[:12], logits[:12], None if log_sum is None else log_sum[:12])
+    for gradient in (False, True):
+        got = backend.distill(scores, teacher, gradient=gradient)
+        check_distill(scores[:12], some, type(got)(got.loss[:12], got.gradient[:12] if gradient else None), type_=type_)
