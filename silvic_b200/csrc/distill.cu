@@ -33,6 +33,12 @@ constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the
 
 constexpr uint32_t kBits = 65536;    // marks of a share: entries past so many share them
 
+// What the derivatives of a list's entries share: with e = exp((z - m) / T) and p = inv_s e, the gradient is slope e
+// outside the top and top_slope e less q in it, the hessian curve p (1 - p).
+struct Slopes {
+    float inv_s, slope, top_slope, curve;
+};
+
 // What a CTA keeps of its share of a list beside the scores.
 template <int kThreads>
 struct Shared {
@@ -42,6 +48,9 @@ struct Shared {
     float q[kMaxTop];
     uint32_t again;                  // some entry's mark was set before
     int32_t far;                     // far scores in the share
+    Slopes slopes;                   // what one warp makes of the sums, for the others
+    float joined_m, q_scale;
+    int32_t empty;
     uint32_t edge_bits;              // marks of the scalars outside the vectors
 };
 
@@ -61,12 +70,6 @@ __device__ __forceinline__ float max_of(const float (&part)[kThreads / 32]) {
     for (int o = kThreads / 64; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
-
-// What the derivatives of a list's entries share: with e = exp((z - m) / T) and p = inv_s e, the gradient is slope e
-// outside the top and top_slope e less q in it, the hessian curve p (1 - p).
-struct Slopes {
-    float inv_s, slope, top_slope, curve;
-};
 
 // Writes an entry's derivatives; the objective's row weight and maxima come in here.
 struct Maxima {
@@ -213,29 +216,49 @@ __device__ __forceinline__ uint32_t marks_of(const Shared<kThreads>& s, const ui
     return m;
 }
 
-// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). `data` holds `slots` vectors
-// (scores, for kVec 1), then the marks: where the share is no longer, it stays there.
+// What is on its way for a CTA's next list while this one's gradients are written.
+struct Ahead {
+    bool flying = false;  // the scores, into the threads' slots, and the thread's entry of the teacher
+    int32_t id;
+    float y;
+};
+
+// The vectors of a list that one of `shares` CTAs (a power of two) takes.
+template <class T, int kVec, bool kCluster>
+__device__ __forceinline__ void share_of(const Walk<T, kVec>& w, uint32_t share, uint32_t shares, uint32_t& from, uint32_t& to) {
+    from = 0;
+    to = w.vectors;
+    if constexpr (kCluster) {
+        const uint32_t shift = __ffs(shares) - 1;
+        from = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * share) >> shift);
+        to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
+    }
+}
+
+// One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). `data` holds `slots` vectors:
+// where the share is no longer, it stays there, each vector in a slot of the thread that reads it. A slot is free once
+// its gradient is written, so list `next` (no list from a.l.lists on) follows through the same slots at once.
 template <class T, int kVec, int kThreads, bool kCluster>
 __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>* data, uint32_t slots, uint32_t* bits,
-                                             const DistillArgs& a, uint32_t i, uint32_t share, uint32_t shares, Maxima& most) {
+                                             const DistillArgs& a, uint32_t i, uint32_t next, Ahead& ahead, uint32_t share,
+                                             uint32_t shares, Maxima& most) {
     constexpr int kUnroll = kVec == 1 ? 4 : 2;
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
     uint64_t first;
     uint32_t n;
     list_range(a.l, i, first, n);
     const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
-    uint32_t from = 0, to = w.vectors;
-    if constexpr (kCluster) {  // shares is a power of two
-        const uint32_t shift = __ffs(shares) - 1;
-        from = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * share) >> shift);
-        to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
-    }
+    uint32_t from, to;
+    share_of<T, kVec, kCluster>(w, share, shares, from, to);
     const float c = __fmul_rn(kLog2E, a.inv_t);
     const bool rest = a.t.log_sum != nullptr;
     const bool held_here = kVec == 1 || to - from <= slots;
+    const float log_sum = rest ? a.t.log_sum[i] : 0.0f, weight = a.weight != nullptr ? a.weight[i] : 1.0f;
     // The scores, on their way to the thread's own slots.
-    if (kVec > 1 && held_here) {
-        for (uint32_t v = from + t; v < to; v += kThreads) data[v - from].copy(w.z + w.at(v));
+    if (kVec > 1 && held_here && !ahead.flying) {
+        const T* z = w.z + w.at(from);
+#pragma unroll 4
+        for (uint32_t v = t; v < to - from; v += kThreads) data[v].copy(z + static_cast<size_t>(v) * kVec);
         copies_begun();
     }
     const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
@@ -244,9 +267,15 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     int32_t id = -1;
     float y = -CUDART_INF_F, zt = -CUDART_INF_F;
     if (t < a.t.top) {
-        teacher_entry(a, i, t, n, id, y);
+        if (ahead.flying) {
+            id = ahead.id;
+            y = ahead.y;
+        } else {
+            teacher_entry(a, i, t, n, id, y);
+        }
         if (id >= 0) zt = to_float(w.z[id]);
     }
+    ahead.flying = false;
     if (t < kMaxTop) s.id[t] = id;
     const uint32_t words = held_here ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
     for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
@@ -344,7 +373,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     bool leads = mine, alone = true;  // the first of the teacher's entries that names this index, and the only one
     if (s.again != 0 && t < a.t.top) lead(s, id, t, a.t.top, leads, alone);
     // The teacher's terms, not yet divided by their sum where the top is all of it.
-    const float base = rest ? a.t.log_sum[i] : y_max;
+    const float base = rest ? log_sum : y_max;
     float q = id >= 0 ? expf(y - base) : 0.0f;
     sum = warp_sum(sum);
     if (lane == 0) s.warp[2][warp] = sum;
@@ -362,12 +391,16 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         s.warp[3][warp] = s.warp[4][warp] = s.warp[5][warp] = 0.0f;
     }
     __syncthreads();
-    // About m itself: the rounding of R is put back.
-    const float settle = far ? 1.0f : pow2(-__fmaf_rn(m, c, -R));
-    float outside = settle * sum_of<kThreads>(s.warp[2]);
-    float top_sum = settle * sum_of<kThreads>(s.warp[3]);
-    float held = sum_of<kThreads>(s.warp[4]);
-    float cross = sum_of<kThreads>(s.warp[5]);
+    // The rest of the scalars are one warp's work.
+    float outside = 0.0f, top_sum = 0.0f, held = 0.0f, cross = 0.0f;
+    if (warp == 0) {
+        // About m itself: the rounding of R is put back.
+        const float settle = far ? 1.0f : pow2(-__fmaf_rn(m, c, -R));
+        outside = settle * sum_of<kThreads>(s.warp[2]);
+        top_sum = settle * sum_of<kThreads>(s.warp[3]);
+        held = sum_of<kThreads>(s.warp[4]);
+        cross = sum_of<kThreads>(s.warp[5]);
+    }
     if constexpr (kCluster) {
         // Every share's sum is about its own reference: their sum is about the largest.
         cg::cluster_group cluster = cg::this_cluster();
@@ -377,56 +410,77 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
             s.top = top_sum;
         }
         cluster.sync();
-        const auto* other = cluster.map_shared_rank(&s, lane & (shares - 1));
-        const float other_m = other->m, other_outside = other->outside, other_top = other->top;
-        float all = other_m;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFull, all, o));
-        const float f = pow2(exponent(other_m, all, c));
-        outside = lane < shares ? other_outside * f : 0.0f;
-        top_sum = lane < shares ? other_top * f : 0.0f;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            outside += __shfl_xor_sync(kFull, outside, o);
-            top_sum += __shfl_xor_sync(kFull, top_sum, o);
+        if (warp == 0) {
+            const auto* other = cluster.map_shared_rank(&s, lane & (shares - 1));
+            const float other_m = other->m, other_outside = other->outside, other_top = other->top;
+            const float all = warp_max(other_m), f = pow2(exponent(other_m, all, c));
+            outside = warp_sum(lane < shares ? other_outside * f : 0.0f);
+            top_sum = warp_sum(lane < shares ? other_top * f : 0.0f);
+            cross += held * ((all - m) * a.inv_t);
+            m = all;
         }
-        outside = __shfl_sync(kFull, outside, 0);
-        top_sum = __shfl_sync(kFull, top_sum, 0);
-        cluster.barrier_arrive();  // the shares' memory is read
-        cross += held * ((all - m) * a.inv_t);
-        m = all;
+    }
+    if (warp == 0) {
+        sum = outside + top_sum;
+        float q_scale = 1.0f;
+        if (!rest && held != 0.0f) {
+            q_scale = 1.0f / held;
+            cross = cross * q_scale - logf(held);
+            held = 1.0f;
+        }
+        const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+        const bool none = sum == 0.0f || !taught;
+        // What the derivatives outside the top share, and what the same formula gives in it.
+        Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
         R = __fmul_rn(m, c);
-        far = !(fabsf(R) < kFar) || !held_here;
+        if (fabsf(R) < kFar && held_here) {  // the terms are about R
+            const float f = pow2(-__fmaf_rn(m, c, -R));
+            k.inv_s *= f;
+            k.slope *= f;
+            k.top_slope *= f;
+        }
+        if (lane == 0) {
+            s.slopes = k;
+            s.joined_m = m;
+            s.q_scale = q_scale;
+            s.empty = none;
+            if (share == 0 && a.loss != nullptr) a.loss[i] = none ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+        }
     }
-    sum = outside + top_sum;
-    float q_scale = 1.0f;
-    if (!rest && held != 0.0f) {
-        q_scale = 1.0f / held;
-        cross = cross * q_scale - logf(held);
-        held = 1.0f;
-    }
-    q *= q_scale;
-    const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
-    const bool empty = sum == 0.0f || !taught;
-    const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
-    if (t == 0 && share == 0 && a.loss != nullptr) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+    __syncthreads();
+    if constexpr (kCluster) cg::this_cluster().barrier_arrive();  // the shares' memory is read
     if (a.grad == nullptr && a.hess == nullptr) {
         if constexpr (kCluster) cg::this_cluster().barrier_wait();
         return;
     }
-    // The derivatives outside the top, and what the same formula gives in it.
-    Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
-    if (!far) {  // the terms are about R
-        const float f = pow2(-__fmaf_rn(m, c, -R));
-        k.inv_s *= f;
-        k.slope *= f;
-        k.top_slope *= f;
-    }
+    m = s.joined_m;
+    R = __fmul_rn(m, c);
+    far = !(fabsf(R) < kFar) || !held_here;
+    const Slopes k = s.slopes;
+    const float q_scale = s.q_scale;
+    const bool empty = s.empty != 0;
+    q *= q_scale;
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
     auto put_one = [&](float z, uint32_t j, bool counts) {
         const float e = empty ? 0.0f : term(z), q_j = e * k.inv_s;
         put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * e, empty ? 0.0f : k.curve * q_j * (1.0f - q_j), counts, most);
     };
+    // The next list's scores follow into each slot as its gradient is written.
+    const T* next_z = nullptr;
+    uint32_t next_count = 0, done = 0;
+    if (kVec > 1 && next < a.l.lists) {
+        uint64_t next_first;
+        uint32_t next_n, next_from, next_to;
+        list_range(a.l, next, next_first, next_n);
+        const Walk<T, kVec> next_w(static_cast<const T*>(a.l.scores) + next_first, next_n);
+        share_of<T, kVec, kCluster>(next_w, share, shares, next_from, next_to);
+        if (next_to - next_from <= slots) {
+            next_z = next_w.z + next_w.at(next_from);
+            next_count = next_to - next_from;
+            ahead.flying = true;
+            if (t < a.t.top) teacher_entry(a, next, t, next_n, ahead.id, ahead.y);
+        }
+    }
     if (!far && !empty) {
         T* const grad = a.grad != nullptr ? static_cast<T*>(a.grad) + out + w.at(from) : nullptr;
         T* const hess = a.hess != nullptr ? static_cast<T*>(a.hess) + out + w.at(from) : nullptr;
@@ -449,7 +503,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                 if (hess != nullptr) hess[v] = from_float<T>(k.curve * p_j * (1.0f - p_j));
             }
         } else if (kVec > 1 && aligned && grad != nullptr && hess == nullptr) {
-#pragma unroll 2
+#pragma unroll kUnroll
             for (uint32_t v = t; v < to - from; v += kThreads) {
                 float x[kVec];
                 get(v, x);
@@ -460,8 +514,12 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                     x[e] = g.x;
                     x[e + 1] = g.y;
                 }
-                if constexpr (kVec > 1) __stcs(reinterpret_cast<uint4*>(grad) + v, packed<T, kVec>(x));
+                if constexpr (kVec > 1) {
+                    __stcs(reinterpret_cast<uint4*>(grad) + v, packed<T, kVec>(x));
+                    if (v < next_count) data[v].copy(next_z + static_cast<size_t>(v) * kVec);
+                }
             }
+            done = to - from;
         } else {
             for (uint32_t v = t; v < to - from; v += kThreads) {
                 float x[kVec], g[kVec], h[kVec];
@@ -493,6 +551,11 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         }
     }
     if (edge_at < n) put_one(edge, edge_at, !edge_marked);
+    if constexpr (kVec > 1) {
+        for (uint32_t v = t; v < next_count; v += kThreads)
+            if (v >= done) data[v].copy(next_z + static_cast<size_t>(v) * kVec);
+        copies_begun();
+    }
     __syncthreads();
     // The top's own, over them.
     if (leads && !empty) {
@@ -519,14 +582,11 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
     uint32_t n;
     list_range(a.l, i, first, n);
     const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
-    uint32_t from = 0, to = w.vectors;
-    if constexpr (kCluster) {
-        const uint32_t shift = __ffs(shares) - 1;
-        from = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * share) >> shift);
-        to = static_cast<uint32_t>((static_cast<uint64_t>(w.vectors) * (share + 1)) >> shift);
-    }
+    uint32_t from, to;
+    share_of<T, kVec, kCluster>(w, share, shares, from, to);
     const float c = __fmul_rn(kLog2E, a.inv_t);
     const bool rest = a.t.log_sum != nullptr;
+    const float log_sum = rest ? a.t.log_sum[i] : 0.0f, weight = a.weight != nullptr ? a.weight[i] : 1.0f;
     Pack<T, kVec> p[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -576,9 +636,11 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
             for (int u = 0; u < kBatch; ++u) {
                 const uint32_t v = base + u * kThreads + t;
                 if (v < to) {
+                    const float high = p[u].most();
                     p[u].values(x);
                     const uint32_t next = v + kBatch * kThreads;
                     if (next < to) p[u].load(w.z + w.at(next));
+                    if (high > r.limit) r.raise(high);
                     const uint32_t skip = look ? marks_of(s, bits, true, w, from, to, a.t.top, v) : 0;
                     if (skip != 0) {
 #pragma unroll
@@ -594,11 +656,14 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
         read(true);
     else
         read(false);
-    if (edge_at < n && !(rest && ((s.edge_bits >> t) & 1u) != 0)) r.add(edge);
+    if (edge_at < n && !(rest && ((s.edge_bits >> t) & 1u) != 0)) {
+        if (edge[0] > r.limit) r.raise(edge[0]);
+        r.add(edge);
+    }
     // The teacher's terms about the first reference, the sums about the largest.
     m = fmaxf(m, -FLT_MAX);
-    const float base = rest ? a.t.log_sum[i] : y_max;
-    Stats mine_sum = settled(r.x, c);
+    const float base = rest ? log_sum : y_max;
+    Stats mine_sum = r.stats();
     const float warp_m = warp_max(mine_sum.m);
     rebase(mine_sum, warp_m, c);
     const float sum_part = warp_sum(mine_sum.s);
@@ -656,7 +721,6 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
         }
         const float sum = outside + top_sum;
         const float rest_q = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
-        const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
         a.loss[i] = sum == 0.0f || !taught ? 0.0f : weight * loss_of(cross, held, sum, outside, rest_q);
     }
     return true;
@@ -672,7 +736,8 @@ __global__ void __launch_bounds__(kThreads) distill_loss_kernel(DistillArgs a, u
     if (loss_list<T, kVec, kThreads, kCluster>(s, bits, a, i, share, shares)) return;
     __syncthreads();
     Maxima most;
-    distill_list<T, kVec, kThreads, kCluster>(s, nullptr, 0, bits, a, i, share, shares, most);
+    Ahead ahead;
+    distill_list<T, kVec, kThreads, kCluster>(s, nullptr, 0, bits, a, i, a.l.lists, ahead, share, shares, most);
 }
 
 template <class T, int kVec, int kThreads, bool kCluster>
@@ -683,8 +748,12 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(
     Maxima most;
     Pack<T, kVec>* data = reinterpret_cast<Pack<T, kVec>*>(held);
     uint32_t* bits = reinterpret_cast<uint32_t*>(held + ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)));
-    const uint32_t shift = kCluster ? __ffs(shares) - 1 : 0;
-    distill_list<T, kVec, kThreads, kCluster>(s, data, slots, bits, a, blockIdx.x >> shift, blockIdx.x & (shares - 1), shares, most);
+    const uint32_t shift = kCluster ? __ffs(shares) - 1 : 0, step = gridDim.x >> shift;
+    Ahead ahead;
+    for (uint32_t i = blockIdx.x >> shift; i < a.l.lists; i += step) {
+        distill_list<T, kVec, kThreads, kCluster>(s, data, slots, bits, a, i, i + step, ahead, blockIdx.x & (shares - 1), shares, most);
+        __syncthreads();  // what the list left in shared memory is read
+    }
     publish<kThreads>(a, most);
 }
 
@@ -854,7 +923,8 @@ __global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillA
         for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
             list_range(a.l, k, first, n);
             if (n <= kWarpEntries) continue;
-            distill_list<T, 1, kWarpThreads, false>(shared, nullptr, 0, bits, a, k, 0, 1, most);
+            Ahead ahead;
+            distill_list<T, 1, kWarpThreads, false>(shared, nullptr, 0, bits, a, k, a.l.lists, ahead, 0, 1, most);
             __syncthreads();
         }
     publish<kWarpThreads>(a, most);
@@ -868,11 +938,12 @@ size_t rows_smem(uint32_t slots) {
     return ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)) + (std::min<size_t>(entries, kBits) + 31) / 32 * 4;
 }
 
-// A launch of `shares` CTAs a list, as clusters where that is more than one.
+// A launch of `shares` CTAs for each of `lists` lists at a time, as clusters where that is more than one.
 template <class Kernel, class... Args>
-void launch_shares(Kernel* kernel, const DistillArgs& a, int threads, size_t smem, uint32_t shares, cudaStream_t s, Args... args) {
+void launch_shares(Kernel* kernel, const DistillArgs& a, uint32_t lists, int threads, size_t smem, uint32_t shares, cudaStream_t s,
+                   Args... args) {
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(a.l.lists * shares);
+    config.gridDim = dim3(lists * shares);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = s;
@@ -889,14 +960,22 @@ void launch_shares(Kernel* kernel, const DistillArgs& a, int threads, size_t sme
 
 template <class T, int kVec, int kThreads>
 void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStream_t s) {
+    const size_t smem = rows_smem<T, kVec>(slots);
+    // CTAs alone that hold their lists: as many as the SMs hold (by threads and registers 768 threads' worth, by shared
+    // memory 227 KB), each taking its next list while it writes.
+    uint32_t lists = a.l.lists;
+    if (kVec > 1 && shares == 1) {
+        const uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(768 / kThreads, 227 * 1024 / (smem + sizeof(Shared<kThreads>) + 1024)));
+        lists = std::min(lists, a.sms * std::max(1u, ctas));
+    }
     launch_shares(shares > 1 ? distill_rows_kernel<T, kVec, kThreads, true> : distill_rows_kernel<T, kVec, kThreads, false>, a,
-                  kThreads, rows_smem<T, kVec>(slots), shares, s, slots);
+                  lists, kThreads, smem, shares, s, slots);
 }
 
 template <class T, int kVec, int kThreads>
 void launch_loss(const DistillArgs& a, uint32_t shares, uint64_t entries, cudaStream_t s) {
     launch_shares(shares > 1 ? distill_loss_kernel<T, kVec, kThreads, true> : distill_loss_kernel<T, kVec, kThreads, false>, a,
-                  kThreads, static_cast<size_t>(std::min<uint64_t>(entries / shares + kVec, kBits) / 32 + 1) * 4, shares, s);
+                  a.l.lists, kThreads, static_cast<size_t>(std::min<uint64_t>(entries / shares + kVec, kBits) / 32 + 1) * 4, shares, s);
 }
 
 template <class T>

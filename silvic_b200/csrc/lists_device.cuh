@@ -84,6 +84,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // score's exponent is finite, so that 0 times it is 0.
 __device__ __forceinline__ float exponent(float z, float m, float c) { return max_nan(__fmul_rn(__fsub_rn(z, m), c), -200.0f); }
 
+// What stands for a masked entry where its exponent is multiplied: its weight is 0 beside any score that is not far.
+constexpr float kMasked = -1.0e30f;
+
 // A list as one thread block (or a cluster of them) walks it: scalars up to the first 16-byte boundary, vectors of
 // kVec entries, scalars behind the last. kVec 1: entry by entry, so that sums do not depend on where a list starts.
 template <class T, int kVec>
@@ -137,6 +140,35 @@ struct Pack {
             }
         }
     }
+    // The largest entry (a NaN gives way).
+    __device__ __forceinline__ float most() const {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+        } else {
+            const uint32_t m = larger(larger(raw.x, raw.y), larger(raw.z, raw.w));
+            if constexpr (std::is_same_v<T, __nv_bfloat16>)
+                return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&m));
+            return fmaxf(v.x, v.y);
+        }
+    }
+    // The entries, masked ones and those of no weight beside scores that are not far as kMasked.
+    __device__ __forceinline__ void finite(float (&f)[kVec]) const {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            Pack p;
+            p.raw = make_uint4(at_least(raw.x), at_least(raw.y), at_least(raw.z), at_least(raw.w));
+            p.values(f);
+        } else {
+            values(f);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) f[e] = max_nan(f[e], kMasked);
+        }
+    }
+    __device__ __forceinline__ static uint32_t at_least(uint32_t a) {
+        const __nv_bfloat162 low = __floats2bfloat162_rn(kMasked, kMasked);
+        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), low);
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
     // The larger of each entry and its counterpart (a NaN gives way).
     __device__ __forceinline__ void raise(const Pack& o) {
         if constexpr (sizeof(T) == 4) {
@@ -177,6 +209,8 @@ struct Pack<T, 1> {
             raw = __ldg(p);
     }
     __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = to_float(raw); }
+    __device__ __forceinline__ float most() const { return to_float(raw); }
+    __device__ __forceinline__ void finite(float (&f)[1]) const { f[0] = max_nan(to_float(raw), kMasked); }
     __device__ __forceinline__ void raise(const Pack& o) { raw = to_float(o.raw) > to_float(raw) || raw != raw ? o.raw : raw; }
     __device__ __forceinline__ void masked() { raw = from_float<T>(-CUDART_INF_F); }
 };
@@ -231,31 +265,27 @@ struct Reader {
         x.r = m == -CUDART_INF_F ? 0.0f : __fmul_rn(m, scale);
     }
     __device__ __forceinline__ bool far() const { return !(fabsf(x.r) < kFar); }
-    // Adds entries; their maximum.
+    __device__ __forceinline__ Stats stats() const { return settled(x, c); }
+    // For entries above the limit (`most` their maximum), before they are added.
+    __device__ __forceinline__ void raise(float most) {
+        x = moved(x, most, c);
+        limit = most + kSlack / c;
+    }
+    // Adds entries up to the limit; kParts: none below kMasked, so that 0 times its exponent is 0.
     template <int kCount>
-    __device__ __forceinline__ float add(const float (&z)[kCount]) {
-        float most = z[0];
-#pragma unroll
-        for (int e = 1; e < kCount; ++e) most = fmaxf(most, z[e]);
-        if (most > limit) {
-            x = moved(x, most, c);
-            limit = most + kSlack / c;
-        }
+    __device__ __forceinline__ void add(const float (&z)[kCount]) {
         if constexpr (kCount == 1) {
-            const float y = max_nan(__fmaf_rn(z[0], c, -x.r), -200.0f), p = pow2(y);
+            const float y = __fmaf_rn(z[0], c, -x.r), p = pow2(y);
             x.a.s += p;
             if (kParts) x.a.v = __fmaf_rn(p, y, x.a.v);
         } else {
-            // pairs in one instruction: issue bounds the kernel before memory
+            // Pairs in one instruction: issue bounds the kernels before memory. A vector's own sums, so that vectors do
+            // not wait for one another.
             const float2 cc = make_float2(c, c), minus_r = make_float2(-x.r, -x.r);
             float2 sum = make_float2(0.0f, 0.0f), part = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int e = 0; e < kCount; e += 2) {
-                float2 y = __ffma2_rn(make_float2(z[e], z[e + 1]), cc, minus_r);
-                if (kParts) {  // a masked entry's 0 times its exponent is 0
-                    y.x = max_nan(y.x, -200.0f);
-                    y.y = max_nan(y.y, -200.0f);
-                }
+                const float2 y = __ffma2_rn(make_float2(z[e], z[e + 1]), cc, minus_r);
                 const float2 p = make_float2(pow2(y.x), pow2(y.y));
                 sum = __fadd2_rn(sum, p);
                 if (kParts) part = __ffma2_rn(p, y, part);
@@ -263,7 +293,6 @@ struct Reader {
             x.a.s += sum.x + sum.y;
             if (kParts) x.a.v += part.x + part.y;
         }
-        return most;
     }
 };
 

@@ -260,10 +260,13 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
             const uint32_t v = base + u * kThreads + t;
             if (v < to) {
                 float x[kVec];
-                p[u].values(x);
+                const float high = p[u].most();
+                p[u].finite(x);
                 const uint32_t next = v + kBatch * kThreads;
                 if (next < to) p[u].load(w.z + w.at(next));
-                if (r.add(x) >= bound) hold(w.at(v));
+                if (high > r.limit) r.raise(high);
+                r.add(x);
+                if (high >= bound) hold(w.at(v));
             }
         }
         // Each time the part that is read has doubled: many candidates are cut to the alternatives so far, whose last
@@ -280,9 +283,14 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
             __syncthreads();
         }
     }
-    if (edge_at < n && r.add(edge) >= bound) hold(edge_at | kSingle);
+    if (edge_at < n) {
+        if (edge[0] > r.limit) r.raise(edge[0]);
+        if (edge[0] >= bound) hold(edge_at | kSingle);
+        edge[0] = max_nan(edge[0], kMasked);
+        r.add(edge);
+    }
     // The share's statistics.
-    Stats mine = settled(r.x, c);
+    Stats mine = r.stats();
     if (__syncthreads_or(r.far())) mine = far_stats<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, c);
     const float top_m = warp_max(mine.m);
     rebase(mine, top_m, c);
