@@ -7,9 +7,9 @@
 //
 // Lists of at most kWarpEntries take a warp each, in registers. Longer ones take a CTA (few of them: a cluster of
 // CTAs), which reads the list once: the maxima of the first batch give the reference, a bound that at least `top`
-// entries reach, and so a filter; entries that pass it are gathered in shared memory and ranked at the end. A list
-// whose order defeats the filter (more candidates than the buffer holds) has its alternatives selected again, digit by
-// digit of their keys.
+// entries reach, and so a filter; vectors that pass it are held in shared memory, their entries cut to the alternatives
+// so far each time the read part has doubled, and ranked at the end. More candidates than the buffer holds (a list in
+// ascending order, or of equal scores) have the alternatives selected digit by digit of their keys.
 #include "lists_device.cuh"
 
 namespace cg = cooperative_groups;
@@ -94,7 +94,7 @@ __device__ __forceinline__ void for_share(const Walk<T, kVec>& w, uint32_t from,
 }
 
 // The share's `top`-th largest key, digit by digit, then the keys from it on: exactly `top` candidates, whatever the
-// order or the ties. The share holds more unmasked entries than kCandidates.
+// order or the ties. The share holds at least as many unmasked entries.
 template <class T, int kVec, int kThreads>
 __device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, uint32_t n, uint32_t from, uint32_t to, bool edges,
                                                uint32_t top) {
@@ -107,8 +107,16 @@ __device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, 
         __syncthreads();
         for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
             const unsigned long long key = order_key(x, j);
-            if (x > -CUDART_INF_F && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
-                atomicAdd(&s.order[static_cast<uint32_t>(key >> shift) & 255u], 1u);
+            if (x > -CUDART_INF_F && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))) {
+                // Equal scores share their digits: one addition for the lanes that are here.
+                const uint32_t d = static_cast<uint32_t>(key >> shift) & 255u, lanes = __activemask();
+                int same;
+                __match_all_sync(lanes, d, &same);
+                if (same == 0)
+                    atomicAdd(&s.order[d], 1u);
+                else if ((threadIdx.x & 31) == static_cast<uint32_t>(__ffs(lanes)) - 1)
+                    atomicAdd(&s.order[d], static_cast<uint32_t>(__popc(lanes)));
+            }
         });
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -169,7 +177,7 @@ __device__ __forceinline__ bool expand(Shared<kThreads>& s, const T* z, float bo
         const uint32_t j = (held & ~kSingle) + e;
         if ((held & kSingle) != 0 && e > 0) continue;
         const float x = to_float(z[j]);
-        if (x >= bound) {
+        if (x >= bound || (held & kSingle) != 0) {
             const uint32_t at = take(&s.keys);
             if (at < kCandidates) s.key[at] = order_key(x, j);
         }
@@ -211,12 +219,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     if (edge_at < n) edge[0] = to_float(w.z[edge_at]);
     float most = edge[0];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-        float x[kVec];
-        p[u].values(x);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) most = fmaxf(most, x[e]);
-    }
+    for (int u = 0; u < kBatch; ++u) most = fmaxf(most, p[u].most());
     // Groups of threads: `top` groups reach the top-th largest of their maxima, so `top` entries do.
     const uint32_t groups = min(static_cast<uint32_t>(kThreads), a.top > 64 ? 256u : 128u), per = kThreads / groups;
     float group = most;
@@ -244,7 +247,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     }
     __syncthreads();
     // Masked entries are no alternatives.
-    float bound = a.top > 0 ? fmaxf(score_of(s.bound), -FLT_MAX) : CUDART_NAN_F;
+    float bound = a.top > 0 ? fmaxf(score_of(s.bound), -FLT_MAX) : CUDART_NAN_F, tie = bound;
     // One pass: the statistics about the first batch's maximum (moved where later entries lie far above it), and the
     // entries that reach the bound.
     Reader<true> r(most, c);
@@ -270,14 +273,17 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
             }
         }
         // Each time the part that is read has doubled: many candidates are cut to the alternatives so far, whose last
-        // is the bound from here on. So candidates stay few however long the list is, unless its order defeats that.
+        // the rest has to exceed (an equal score further on comes after it). So candidates stay few however long the
+        // list is and however many scores are equal, unless its order defeats that.
         if ((++batch & (batch - 1)) == 0 && a.top > 0 && base + kBatch * kThreads < to) {
             __syncthreads();
             if (s.count > max(64u, 2 * a.top) && expand<T, kVec, kThreads>(s, w.z, bound)) {
                 rank_candidates(s, s.keys, a.top);
                 __syncthreads();
                 for (uint32_t k = t; k < a.top; k += kThreads) s.held[k] = index_of(s.best[k]) | kSingle;
-                bound = score_of(static_cast<uint32_t>(s.best[a.top - 1] >> 32));
+                const uint32_t last = static_cast<uint32_t>(s.best[a.top - 1] >> 32);
+                tie = score_of(last);
+                bound = score_of(last + 1);
                 if (t == 0) s.count = a.top;
             }
             __syncthreads();
@@ -285,7 +291,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     }
     if (edge_at < n) {
         if (edge[0] > r.limit) r.raise(edge[0]);
-        if (edge[0] >= bound) hold(edge_at | kSingle);
+        if (edge[0] >= tie) hold(edge_at | kSingle);
         edge[0] = max_nan(edge[0], kMasked);
         r.add(edge);
     }

@@ -634,3 +634,23 @@ def test_distill_of_far_scores(backend, lists, width, type_, rest):
     for gradient in (False, True):
         got = backend.distill(scores, teacher, gradient=gradient)
         check_distill(scores[:12], some, type(got)(got.loss[:12], got.gradient[:12] if gradient else None), type_=type_)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("width,pad", [(700, 0), (9001, 3), (40000, 0), (150001, 0)])
+def test_log_probs_of_equal_scores(backend, type_, width, pad):
+    """Lists of a few distinct scores, whole lists of one score among them: ties go to the lower index."""
+    rng = np.random.RandomState(width)
+    scores = dense(rng, 300, width, type_, pad)
+    scores[:] = torch.from_numpy(rng.randint(0, 3, (300, width))).to(scores.dtype).cuda()
+    scores[0] = 0.5
+    scores[1] = -4.0
+    scores[1, width - 1] = 1.0
+    scores[2, ::2] = -np.inf
+    scores[3] = torch.arange(width, device="cuda").float() / width * 3
+    ids = torch.zeros(300, 1, dtype=torch.int32, device="cuda")
+    for some in (scores, scores[:5]):  # a CTA a list; clusters
+        for top in (1, 40, 128):
+            got = backend.log_probs(some, given=ids[: len(some)], top=top)
+            check_log_probs(some[:5], rows_of(some[:5]), host(ids)[:5].astype(int), top, 1.0,
+                            type(got)(*[v[:5] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
