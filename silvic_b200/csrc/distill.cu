@@ -203,8 +203,12 @@ __device__ __forceinline__ uint32_t marks_of(const Shared<kThreads>& s, const ui
                                              uint32_t from, uint32_t to, uint32_t top, uint32_t v) {
     uint32_t m = ~0u;
     if (room) {
-        const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
-        m = (bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
+        if constexpr (kVec == 8) {  // a byte a vector
+            m = reinterpret_cast<const uint8_t*>(bits)[(v - from) & (kBits / 8 - 1)];
+        } else {
+            const uint32_t bit = ((v - from) * kVec) & (kBits - 1);
+            m = (bits[bit / 32] >> (bit & 31)) & ((1u << kVec) - 1u);
+        }
     }
     if (m != 0 && (!room || (to - from) * kVec > kBits)) {
         m = 0;
