@@ -796,7 +796,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     }
     int32_t id[kTop];
     float y[kTop], zt[kTop], y_max = -CUDART_INF_F;
-    bool taught = false;
+    bool taught = false, again = false;
     if (lane < kItems) s.bits[lane] = 0;
     __syncwarp();
 #pragma unroll
@@ -811,7 +811,8 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         if (id[u] >= 0) {
             y[u] = logits[u] * a.inv_t;
             zt[u] = to_float(z[id[u]]);
-            atomicOr(&s.bits[id[u] / 32], 1u << (id[u] & 31));
+            const uint32_t mark = 1u << (id[u] & 31);
+            again |= (atomicOr(&s.bits[id[u] / 32], mark) & mark) != 0;
             taught = true;
         }
         y_max = fmaxf(y_max, y[u]);
@@ -819,6 +820,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     m = fmaxf(warp_max(m), -FLT_MAX);
     y_max = fmaxf(warp_max(y_max), -FLT_MAX);
     taught = __any_sync(kFull, taught);  // and the marks are set
+    again = __any_sync(kFull, again);    // an index named twice
     uint32_t marks = 0;
     float sum = 0.0f;
 #pragma unroll
@@ -834,11 +836,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
 #pragma unroll
     for (int u = 0; u < kTop; ++u) {
         bool first_one = id[u] >= 0, only = true;
-        if (kTop == 1) {
-            const uint32_t same = __match_any_sync(kFull, id[u]);
-            first_one = first_one && static_cast<uint32_t>(__ffs(same) - 1) == lane;
-            only = same == 1u << lane;
-        } else {
+        if (again) {
             for (uint32_t k = 0; k < a.t.top; ++k)
                 if (s.id[k] == id[u] && k != u * 32 + lane) {
                     only = false;

@@ -31,6 +31,7 @@ constexpr int kWarpThreads = 256;        // the warp kernel's CTAs
 constexpr uint32_t kCandidates = 2048;   // keys that a CTA gathers
 constexpr int kBatch = 4;                // vectors a thread holds in flight (2: 286 us above, 4: 246, 8: 258)
 constexpr uint32_t kSingle = 0x80000000u;
+constexpr uint32_t kRanked = 256;        // keys that are ranked by counting
 
 // What a CTA keeps of its share of a list.
 template <int kThreads>
@@ -45,44 +46,107 @@ struct Shared {
     uint32_t count, keys, digit, left;
 };
 
-// The share's `top` largest keys of `count` gathered ones into s.best, in order. Few: every key counts the keys above
-// it; many: a bitonic sort. Ends without a barrier behind the writes of s.best.
-template <int kThreads>
-__device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t count, uint32_t top) {
-    const uint32_t t = threadIdx.x;
-    for (uint32_t i = t; i < top; i += kThreads) s.best[i] = 0;
-    __syncthreads();
-    if (count <= 512) {
-        for (uint32_t i = t; i < count; i += kThreads) {
-            const unsigned long long mine = s.key[i];
-            uint32_t above = 0, j = 0;
-            for (; j + 4 <= count; j += 4) {
-                const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&s.key[j]);
-                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.key[j + 2]);
-                above += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
-            }
-            for (; j < count; ++j) above += s.key[j] > mine;
-            if (above < top) s.best[above] = mine;
+// The next free slot of a buffer in shared memory. Rarely more than one lane of a warp asks, so the plain atomic is
+// cheaper than one for the warp and a share of it per lane.
+__device__ __forceinline__ uint32_t take(uint32_t* counter) {
+    uint32_t at;
+    asm volatile("atom.shared.add.u32 %0, [%1], 1;"
+                 : "=r"(at)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(counter)))
+                 : "memory");
+    return at;
+}
+
+// The `top`-th largest of the keys that `each` hands to its argument (at least `top`, all different), digit by digit:
+// the keys that share the digits so far are counted by the next one. Digits that all keys of `T` scores and of indices
+// below `n` share are known: an index's high ones, and those of a 16-bit score's low half as f32, which its sign sets.
+template <class T, int kThreads, class Each>
+__device__ __forceinline__ unsigned long long nth_key(Shared<kThreads>& s, uint32_t top, uint32_t n, Each each) {
+    unsigned long long prefix = 0;
+    uint32_t left = top;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        const bool score = sizeof(T) == 2 && (shift == 32 || (shift == 40 && std::is_same_v<T, __nv_bfloat16>));
+        if (score || (shift < 32 && shift > 0 && n <= 1u << shift)) {
+            if (!score || (prefix >> 63) == 0) prefix |= 0xFFull << shift;
+            continue;
         }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < 256; i += kThreads) s.order[i] = 0;
+        __syncthreads();
+        each([&](unsigned long long key) {
+            if (shift != 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
+            // Equal scores share their digits: one addition for the lanes that are here.
+            const uint32_t d = static_cast<uint32_t>(key >> shift) & 255u, lanes = __activemask();
+            int same;
+            __match_all_sync(lanes, d, &same);
+            if (same == 0)
+                atomicAdd(&s.order[d], 1u);
+            else if ((threadIdx.x & 31) == static_cast<uint32_t>(__ffs(lanes)) - 1)
+                atomicAdd(&s.order[d], static_cast<uint32_t>(__popc(lanes)));
+        });
+        __syncthreads();
+        if (threadIdx.x < 32) {  // a lane sums 8 digits; the lane whose digits hold the one that is looked for finds it
+            const uint32_t lane = threadIdx.x;
+            uint32_t sum = 0;
+            for (uint32_t k = 0; k < 8; ++k) sum += s.order[255 - 8 * lane - k];
+            uint32_t upto = sum;
+            for (uint32_t o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(kFull, upto, o);
+                if (lane >= o) upto += u;
+            }
+            if (upto >= left && upto - sum < left) {
+                uint32_t need = left - (upto - sum), d = 255 - 8 * lane;
+                while (s.order[d] < need) need -= s.order[d--];
+                s.digit = d;
+                s.left = s.order[d] == need ? 0 : need;  // 0: all keys with these digits belong
+            }
+        }
+        __syncthreads();
+        prefix |= static_cast<unsigned long long>(s.digit) << shift;
+        left = s.left;
+        if (left == 0) break;
+    }
+    return prefix;
+}
+
+// The `top` largest of `count` gathered keys into s.best, in order: every key counts the keys above it, of more than
+// kRanked only the `top` largest (of 512 keys the counting takes 37,000 instructions, finding the top-th 7,000). Ends
+// without a barrier behind the writes of s.best.
+template <class T, int kThreads>
+__device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t count, uint32_t top, uint32_t n) {
+    const uint32_t t = threadIdx.x;
+    if (count > kRanked) {
+        const unsigned long long last = nth_key<T>(s, top, n, [&](auto f) {
+            for (uint32_t i = t; i < count; i += kThreads) f(s.key[i]);
+        });
+        if (t == 0) s.count = 0;
+        __syncthreads();
+        for (uint32_t i = t; i < count; i += kThreads)
+            if (s.key[i] >= last) s.best[take(&s.count)] = s.key[i];
+        __syncthreads();
+        unsigned long long mine = 0;
+        uint32_t above = 0;
+        if (t < top) {
+            mine = s.best[t];
+            for (uint32_t j = 0; j < top; ++j) above += s.best[j] > mine;
+        }
+        __syncthreads();
+        if (t < top) s.best[above] = mine;
         return;
     }
-    uint32_t cap = 1024;
-    while (cap < count) cap <<= 1;
-    for (uint32_t i = count + t; i < cap; i += kThreads) s.key[i] = 0;
+    for (uint32_t i = t; i < top; i += kThreads) s.best[i] = 0;
     __syncthreads();
-    for (uint32_t size = 2; size <= cap; size <<= 1)
-        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-            for (uint32_t x = t; x < cap / 2; x += kThreads) {
-                const uint32_t lo = 2 * x - (x & (stride - 1)), hi = lo + stride;
-                const unsigned long long a = s.key[lo], b = s.key[hi];
-                if ((a < b) == ((lo & size) == 0)) {
-                    s.key[lo] = b;
-                    s.key[hi] = a;
-                }
-            }
-            __syncthreads();
+    for (uint32_t i = t; i < count; i += kThreads) {
+        const unsigned long long mine = s.key[i];
+        uint32_t above = 0, j = 0;
+        for (; j + 4 <= count; j += 4) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&s.key[j]);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.key[j + 2]);
+            above += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
         }
-    for (uint32_t i = t; i < top; i += kThreads) s.best[i] = s.key[i];
+        for (; j < count; ++j) above += s.key[j] > mine;
+        if (above < top) s.best[above] = mine;
+    }
 }
 
 // Entries [from, to) of the vectors and, for share 0, the scalars outside them, each to `f(score, index)`.
@@ -101,60 +165,24 @@ __device__ __forceinline__ void for_share(const Walk<T, kVec>& w, uint32_t from,
     }
 }
 
-// The share's `top`-th largest key, digit by digit, then the keys from it on: exactly `top` candidates, whatever the
-// order or the ties. The share holds at least as many unmasked entries.
+// The share's `top` largest keys as the candidates, whatever the order or the ties. The share holds at least as many
+// unmasked entries.
 template <class T, int kVec, int kThreads>
 __device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, uint32_t n, uint32_t from, uint32_t to, bool edges,
                                                uint32_t top) {
     const Walk<T, kVec> w(z, n);
-    unsigned long long prefix = 0;
-    uint32_t left = top;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 256; i += kThreads) s.order[i] = 0;
-        __syncthreads();
+    auto each = [&](auto f) {
         for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
-            const unsigned long long key = order_key(x, j);
-            if (x > -CUDART_INF_F && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))) {
-                // Equal scores share their digits: one addition for the lanes that are here.
-                const uint32_t d = static_cast<uint32_t>(key >> shift) & 255u, lanes = __activemask();
-                int same;
-                __match_all_sync(lanes, d, &same);
-                if (same == 0)
-                    atomicAdd(&s.order[d], 1u);
-                else if ((threadIdx.x & 31) == static_cast<uint32_t>(__ffs(lanes)) - 1)
-                    atomicAdd(&s.order[d], static_cast<uint32_t>(__popc(lanes)));
-            }
+            if (x > -CUDART_INF_F) f(order_key(x, j));
         });
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t d = 255, need = left;
-            while (d > 0 && s.order[d] < need) need -= s.order[d--];
-            s.digit = d;
-            s.left = need;
-        }
-        __syncthreads();
-        prefix |= static_cast<unsigned long long>(s.digit) << shift;
-        left = s.left;
-    }
+    };
+    const unsigned long long last = nth_key<T>(s, top, n, each);
     if (threadIdx.x == 0) s.keys = 0;
     __syncthreads();
-    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
-        const unsigned long long key = order_key(x, j);
-        if (x > -CUDART_INF_F && key >= prefix) {
-            const uint32_t at = atomicAdd(&s.keys, 1u);
-            if (at < kCandidates) s.key[at] = key;
-        }
+    each([&](unsigned long long key) {
+        if (key >= last) s.key[take(&s.keys)] = key;
     });
     __syncthreads();
-}
-
-// The next free slot of a buffer in shared memory. Rarely more than one lane of a warp asks, so the plain atomic is
-// cheaper than one for the warp and a share of it per lane.
-__device__ __forceinline__ uint32_t take(uint32_t* counter) {
-    uint32_t at;
-    asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(counter))) : "memory");
-    return at;
 }
 
 // The statistics of a share of far scores (about 700,000 T and more from 0): the maximum first, then each entry's
@@ -287,7 +315,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
         if ((++batch & (batch - 1)) == 0 && a.top > 0 && base + kBatch * kThreads < to) {
             __syncthreads();
             if (s.count > max(64u, 2 * a.top) && expand<T, kVec, kThreads>(s, w.z, bound)) {
-                rank_candidates(s, s.keys, a.top);
+                rank_candidates<T>(s, s.keys, a.top, n);
                 __syncthreads();
                 for (uint32_t k = t; k < a.top; k += kThreads) s.held[k] = index_of(s.best[k]) | kSingle;
                 const uint32_t last = static_cast<uint32_t>(s.best[a.top - 1] >> 32);
@@ -330,7 +358,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     if (a.top > 0) {
         if (!expand<T, kVec, kThreads>(s, w.z, bound))
             select_candidates<T, kVec, kThreads>(s, w.z, n, from, to, share == 0, a.top);
-        rank_candidates(s, s.keys, a.top);
+        rank_candidates<T>(s, s.keys, a.top, n);
     }
     __syncthreads();
     if constexpr (kCluster) {
@@ -358,7 +386,7 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
                 if (key != 0) s.key[atomicAdd(&s.keys, 1u)] = key;
             }
             __syncthreads();
-            if (a.top > 0) rank_candidates(s, s.keys, a.top);
+            if (a.top > 0) rank_candidates<T>(s, s.keys, a.top, n);
         }
         cluster.sync();  // the shares' memory is read
         if (share != 0) return;
@@ -435,6 +463,38 @@ __device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i
     unsigned long long key[kItems];
 #pragma unroll
     for (int k = 0; k < kItems; ++k) key[k] = x[k] > -CUDART_INF_F || x[k] != x[k] ? order_key(x[k], k * 32 + lane) : 0ull;
+    if (a.top > 32) {
+        // Many: a bitonic sort of the warp's entries, lane l with places l kItems onwards (369 entries, top 128: rounds
+        // took 30 us).
+#pragma unroll
+        for (int size = 2; size <= 32 * kItems; size <<= 1)
+#pragma unroll
+            for (int stride = size >> 1; stride > 0; stride >>= 1)
+#pragma unroll
+                for (int k = 0; k < kItems; ++k) {
+                    const bool down = ((lane * kItems + k) & size) == 0;  // this stretch: largest first
+                    if (stride >= kItems) {
+                        const unsigned long long other = __shfl_xor_sync(kFull, key[k], stride / kItems);
+                        const bool low = (lane & (stride / kItems)) == 0;
+                        if ((key[k] < other) == (low == down)) key[k] = other;
+                    } else if ((k ^ stride) > k) {
+                        const int o = k ^ stride;
+                        const unsigned long long u = key[k], v = key[o];
+                        const bool swap = (u < v) == down;
+                        key[k] = swap ? v : u;
+                        key[o] = swap ? u : v;
+                    }
+                }
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const uint32_t at_top = lane * kItems + k;
+            if (at_top >= a.top) continue;
+            const uint64_t at = static_cast<uint64_t>(i) * a.top + at_top;
+            a.top_ids[at] = key[k] == 0 ? -1 : static_cast<int32_t>(index_of(key[k]));
+            a.top_out[at] = key[k] == 0 ? -CUDART_INF_F : (score_of(static_cast<uint32_t>(key[k] >> 32)) - m) * a.inv_t - log_s;
+        }
+        return;
+    }
 #pragma unroll
     for (int size = 2; size <= kItems; size <<= 1)  // a bitonic network over the lane's own, largest first
 #pragma unroll
@@ -460,7 +520,7 @@ __device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i
         }
         const uint32_t winner = __ffs(who) - 1;
         const uint32_t won = __shfl_sync(kFull, low, winner);
-        if (lane == (r & 31)) {
+        if (lane == r) {
             out_order = most_order;
             out_low = won;
         }
@@ -469,15 +529,11 @@ __device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i
             for (int k = 0; k + 1 < kItems; ++k) key[k] = key[k + 1];
             key[kItems - 1] = 0;
         }
-        if ((r & 31) == 31 || r + 1 == a.top) {  // 32 alternatives leave together
-            const uint32_t at_top = (r & ~31u) + lane;
-            if (at_top < a.top) {
-                const uint64_t at = static_cast<uint64_t>(i) * a.top + at_top;
-                a.top_ids[at] = out_order == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - out_low);
-                a.top_out[at] = out_order == 0 ? -CUDART_INF_F : (score_of(out_order) - m) * a.inv_t - log_s;
-            }
-            out_order = 0;
-        }
+    }
+    if (lane < a.top) {
+        const uint64_t at = static_cast<uint64_t>(i) * a.top + lane;
+        a.top_ids[at] = out_order == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - out_low);
+        a.top_out[at] = out_order == 0 ? -CUDART_INF_F : (score_of(out_order) - m) * a.inv_t - log_s;
     }
 }
 

@@ -654,3 +654,33 @@ def test_log_probs_of_equal_scores(backend, type_, width, pad):
             got = backend.log_probs(some, given=ids[: len(some)], top=top)
             check_log_probs(some[:5], rows_of(some[:5]), host(ids)[:5].astype(int), top, 1.0,
                             type(got)(*[v[:5] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [32, 33, 100, 128])
+@pytest.mark.parametrize("width", [20, 100, 130, 300, 512, 631, 1100])
+def test_log_probs_of_many_alternatives(backend, type_, top, width):
+    """Short lists with more alternatives than a warp has lanes, masked entries and ties among them."""
+    rng = np.random.RandomState(width + top)
+    scores = dense(rng, 40, width, type_, 1)
+    scores[::3, ::4] = -np.inf
+    scores[::5] = torch.round(scores[::5])
+    got = backend.log_probs(scores, top=top)
+    check_log_probs(scores, rows_of(scores), None, top, 1.0, got)
+
+
+@pytest.mark.parametrize("sizes", [[200, 3, 400, 40], [700, 5000]])
+def test_distill_teachers_that_name_an_entry_twice(backend, sizes):
+    """Tops of more than 32 entries with repeated indices, in the warp's lists and longer ones."""
+    rng = np.random.RandomState(len(sizes))
+    bounds = np.concatenate([[0], np.cumsum(sizes)])
+    scores = torch.from_numpy(rng.randn(bounds[-1])).float().cuda()
+    for rest in (False, True):
+        teacher = random_teacher(rng, sizes, 70, "f32", rest)
+        ids = teacher.ids.clone()
+        ids[:, 65] = ids[:, 1]
+        ids[0, 40] = ids[0, 3]
+        ids[:, 69] = ids[:, 1]
+        teacher = TeacherTop(ids, teacher.logits, teacher.log_sum)
+        got = backend.distill(scores, teacher, boundaries=torch.from_numpy(bounds.astype(np.int32)).cuda(), hessian=True)
+        check_distill(scores, teacher, got, None, bounds)
