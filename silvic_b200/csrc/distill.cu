@@ -38,6 +38,9 @@ namespace sb2 {
 namespace {
 
 constexpr uint32_t kWarpEntries = 512;
+// The mean length up to which runs between boundaries go by warps, the longer ones among them by whole CTAs: 20,000 lists
+// of 300 take 24 us so and 71 by a CTA each; of widely spread lengths about 300, 70 and 75, about 440, 54 and 42.
+constexpr uint32_t kWarpMean = 384;
 constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
 constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
@@ -900,19 +903,19 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     }
 }
 
-// A warp per list; a longer one among them by the whole CTA.
+// `per` lists a CTA (8 at most), a warp each; a longer one among them by the whole CTA. So what a list gives depends on
+// its own length alone.
 template <class T, int kTop>
-__global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillArgs a, uint32_t per) {
     if (a.stopped != nullptr && *a.stopped) return;
-    constexpr uint32_t kLists = kWarpThreads / 32;
-    __shared__ WarpShared warps[kLists];
+    __shared__ WarpShared warps[kWarpThreads / 32];
     __shared__ Shared<kWarpThreads> shared;
     __shared__ uint32_t bits[kBits / 32];
-    const uint32_t base = blockIdx.x * kLists, i = base + (threadIdx.x >> 5);
+    const uint32_t base = blockIdx.x * per, i = base + (threadIdx.x >> 5);
     uint64_t first = 0;
     uint32_t n = 0;
     Maxima most;
-    if (i < a.l.lists) {
+    if (threadIdx.x >> 5 < per && i < a.l.lists) {
         // The teacher's entries, on their way beside the boundaries.
         int32_t ids[kTop];
         float logits[kTop];
@@ -933,7 +936,7 @@ __global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillA
             distill_warp<T, 16, kTop>(s, a, i, first, n, ids, logits, most);
     }
     if (__syncthreads_or(n > kWarpEntries) != 0)
-        for (uint32_t k = base; k < base + kLists && k < a.l.lists; ++k) {
+        for (uint32_t k = base; k < base + per && k < a.l.lists; ++k) {
             list_range(a.l, k, first, n);
             if (n <= kWarpEntries) continue;
             Ahead ahead;
@@ -995,12 +998,13 @@ template <class T>
 void launch_typed(const DistillArgs& a, cudaStream_t s) {
     constexpr int kVec = 16 / sizeof(T);
     const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
-    if (mean <= (a.l.bounds != nullptr ? kWarpEntries / 2 : kWarpEntries)) {
-        const uint32_t lists = kWarpThreads / 32, grid = (a.l.lists + lists - 1) / lists;
+    const bool narrow = mean <= (a.l.bounds != nullptr ? kWarpMean : kWarpEntries);
+    if (narrow || a.max_g != nullptr) {  // a training iteration's queries: the same gradients on any rank
+        const uint32_t per = narrow ? kWarpThreads / 32 : 1, grid = a.l.lists / per + (a.l.lists % per != 0);
         if (a.t.top <= 32)
-            distill_warps_kernel<T, 1><<<grid, kWarpThreads, 0, s>>>(a);
+            distill_warps_kernel<T, 1><<<grid, kWarpThreads, 0, s>>>(a, per);
         else
-            distill_warps_kernel<T, 4><<<grid, kWarpThreads, 0, s>>>(a);
+            distill_warps_kernel<T, 4><<<grid, kWarpThreads, 0, s>>>(a, per);
         return;
     }
     uint32_t shares = list_shares(mean, a.l.lists, a.sms);

@@ -27,6 +27,9 @@ namespace sb2 {
 namespace {
 
 constexpr uint32_t kWarpEntries = 512;
+// The mean length up to which runs between boundaries go by warps, the longer ones among them by whole CTAs: 20,000 lists
+// of 300 to 400 take 61 us so and 94 by a CTA each; of widely spread lengths about 300, 113 and 100.
+constexpr uint32_t kWarpMean = 384;
 constexpr int kWarpThreads = 256;        // the warp kernel's CTAs
 constexpr uint32_t kCandidates = 2048;   // keys that a CTA gathers
 constexpr int kBatch = 4;                // vectors a thread holds in flight (2: 286 us above, 4: 246, 8: 258)
@@ -587,13 +590,15 @@ template <class T>
 void launch_typed(const LogProbsArgs& a, cudaStream_t s) {
     constexpr int kVec = 16 / sizeof(T);
     const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
-    if (mean <= (a.l.bounds != nullptr ? kWarpEntries / 2 : kWarpEntries)) {
+    if (mean <= (a.l.bounds != nullptr ? kWarpMean : kWarpEntries)) {
         const uint32_t lists = kWarpThreads / 32;
         log_probs_warps_kernel<T><<<(a.l.lists + lists - 1) / lists, kWarpThreads, 0, s>>>(a);
         return;
     }
     const uint32_t shares = list_shares(mean, a.l.lists, a.sms);
-    if (a.l.bounds != nullptr)
+    if (a.l.bounds != nullptr && mean <= 1024)  // (10,478 lists of 588: 128 threads 64 us, 256 81; 1500 of 3500: 44 and 33)
+        launch_rows<T, 1, 128>(a, shares, s);
+    else if (a.l.bounds != nullptr)
         launch_rows<T, 1, 256>(a, shares, s);
     else if (mean <= 128 * kBatch * kVec)  // one batch of 128 threads holds the list
         launch_rows<T, kVec, 128>(a, shares, s);

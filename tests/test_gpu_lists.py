@@ -684,3 +684,34 @@ def test_distill_teachers_that_name_an_entry_twice(backend, sizes):
         teacher = TeacherTop(ids, teacher.logits, teacher.log_sum)
         got = backend.distill(scores, teacher, boundaries=torch.from_numpy(bounds.astype(np.int32)).cuda(), hessian=True)
         check_distill(scores, teacher, got, None, bounds)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_objective_gradients_do_not_depend_on_the_shard(device, rest):
+    """Queries of very different lengths: a rank that holds the short ones, or the long ones, has the same bits."""
+    rng = np.random.RandomState(12)
+    sizes = np.array([40] * 30 + [130, 300, 500, 512, 513, 700, 2_000, 6_000, 1, 3_000, 90])
+    bounds = np.concatenate([[0], np.cumsum(sizes)])
+    n = int(bounds[-1])
+    teacher = ranking_teacher(rng, bounds, 20, rest)
+
+    def gradients(first, last):
+        a, b = int(bounds[first]), int(bounds[last])
+        data = ranking_binned(b - a, [31] * 2, seed=8, mean_query=40.0)
+        data.query_boundaries = (bounds[first:last + 1] - a).astype(np.uint32)
+        part = TeacherTop(teacher.ids[first:last], teacher.logits[first:last],
+                          None if teacher.log_sum is None else teacher.log_sum[first:last], teacher.temperature)
+        with B200Backend(device) as back:
+            back.load(data, "distill")
+            back.set_teacher(part)
+            back.init_scores(0, 0.0)
+            back.compute_gradients()
+            return back.read_gradients()
+
+    whole = gradients(0, len(sizes))
+    for first, last in ((0, 30), (30, len(sizes)), (34, 38)):
+        a, b = int(bounds[first]), int(bounds[last])
+        part = gradients(first, last)
+        for x, y in zip(whole, part):
+            assert np.array_equal(x[a:b].view(np.uint32), y.view(np.uint32))
+    assert n == len(whole[0])
