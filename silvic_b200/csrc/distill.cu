@@ -11,7 +11,7 @@
 // little there. The top's entries are marked in a bitmap, which the sum skips; their gradients are written once the
 // others are, over what the common formula left there. An entry named twice has its q added in the teacher's order.
 //
-// Lists of at most kWarpEntries take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
+// Lists of at most 512 entries (1024 of a dense matrix) take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
 // holds it in shared memory between the passes (each thread its own vectors), so that memory sees each score once. Runs
 // between boundaries are read again from the caches, entry by entry, so that a list's sums do not depend on where it
 // starts. A dense list too long for shared memory, or of scores so far from 0 that fma(z, c, -m c) loses its last bits,
@@ -37,7 +37,6 @@ namespace sb2 {
 
 namespace {
 
-constexpr uint32_t kWarpEntries = 512;
 // The mean length up to which runs between boundaries go by warps, the longer ones among them by whole CTAs: 20,000 lists
 // of 300 take 24 us so and 71 by a CTA each; of widely spread lengths about 300, 70 and 75, about 440, 54 and 42.
 constexpr uint32_t kWarpMean = 384;
@@ -777,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(
 
 // A warp's teacher: its marks (a bit an entry of the list), ids and q.
 struct WarpShared {
-    uint32_t bits[kWarpEntries / 32];
+    uint32_t bits[32];
     int32_t id[kMaxTop];
     float q[kMaxTop];
 };
@@ -903,10 +902,11 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     }
 }
 
-// `per` lists a CTA (8 at most), a warp each; a longer one among them by the whole CTA. So what a list gives depends on
+// `per` lists a CTA (8 at most), a warp each of at most 32 kMost entries; a longer one among them by the whole CTA. So what a list gives depends on
 // its own length alone.
-template <class T, int kTop>
-__global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillArgs a, uint32_t per) {
+template <class T, int kTop, int kMost>
+__global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4) distill_warps_kernel(DistillArgs a, uint32_t per) {
+    constexpr uint32_t kEntries = 32 * kMost;
     if (a.stopped != nullptr && *a.stopped) return;
     __shared__ WarpShared warps[kWarpThreads / 32];
     __shared__ Shared<kWarpThreads> shared;
@@ -932,13 +932,15 @@ __global__ void __launch_bounds__(kWarpThreads, 4) distill_warps_kernel(DistillA
             distill_warp<T, 4, kTop>(s, a, i, first, n, ids, logits, most);
         else if (n <= 256)
             distill_warp<T, 8, kTop>(s, a, i, first, n, ids, logits, most);
-        else if (n <= kWarpEntries)
+        else if (n <= 512)
             distill_warp<T, 16, kTop>(s, a, i, first, n, ids, logits, most);
+        else if (n <= kEntries)
+            distill_warp<T, kMost, kTop>(s, a, i, first, n, ids, logits, most);
     }
-    if (__syncthreads_or(n > kWarpEntries) != 0)
+    if (__syncthreads_or(n > kEntries) != 0)
         for (uint32_t k = base; k < base + per && k < a.l.lists; ++k) {
             list_range(a.l, k, first, n);
-            if (n <= kWarpEntries) continue;
+            if (n <= kEntries) continue;
             Ahead ahead;
             distill_list<T, 1, kWarpThreads, false>(shared, nullptr, 0, bits, a, k, a.l.lists, ahead, 0, 1, most);
             __syncthreads();
@@ -998,13 +1000,21 @@ template <class T>
 void launch_typed(const DistillArgs& a, cudaStream_t s) {
     constexpr int kVec = 16 / sizeof(T);
     const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
-    const bool narrow = mean <= (a.l.bounds != nullptr ? kWarpMean : kWarpEntries);
+    const bool narrow = mean <= (a.l.bounds != nullptr ? kWarpMean : 512);
     if (narrow || a.max_g != nullptr) {  // a training iteration's queries: the same gradients on any rank
         const uint32_t per = narrow ? kWarpThreads / 32 : 1, grid = a.l.lists / per + (a.l.lists % per != 0);
         if (a.t.top <= 32)
-            distill_warps_kernel<T, 1><<<grid, kWarpThreads, 0, s>>>(a, per);
+            distill_warps_kernel<T, 1, 16><<<grid, kWarpThreads, 0, s>>>(a, per);
         else
-            distill_warps_kernel<T, 4><<<grid, kWarpThreads, 0, s>>>(a, per);
+            distill_warps_kernel<T, 4, 16><<<grid, kWarpThreads, 0, s>>>(a, per);
+        return;
+    }
+    if (a.l.bounds == nullptr && mean <= 1024) {  // (8000 x 1000 f32: a warp each 21 us, a CTA each 38; 64 of them: 5.4 and 4.7)
+        const uint32_t per = kWarpThreads / 32, grid = a.l.lists / per + (a.l.lists % per != 0);
+        if (a.t.top <= 32)
+            distill_warps_kernel<T, 1, 32><<<grid, kWarpThreads, 0, s>>>(a, per);
+        else
+            distill_warps_kernel<T, 4, 32><<<grid, kWarpThreads, 0, s>>>(a, per);
         return;
     }
     uint32_t shares = list_shares(mean, a.l.lists, a.sms);
