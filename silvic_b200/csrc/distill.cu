@@ -819,9 +819,10 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         }
         y_max = fmaxf(y_max, y[u]);
     }
+    __syncwarp();  // the marks and the ids, which other lanes read (votes and shuffles order no memory)
     m = fmaxf(warp_max(m), -FLT_MAX);
     y_max = fmaxf(warp_max(y_max), -FLT_MAX);
-    taught = __any_sync(kFull, taught);  // and the marks are set
+    taught = __any_sync(kFull, taught);
     again = __any_sync(kFull, again);    // an index named twice
     uint32_t marks = 0;
     float sum = 0.0f;
