@@ -61,7 +61,8 @@ __device__ __forceinline__ uint32_t take(uint32_t* counter) {
 }
 
 // The `top`-th largest of the keys that `each` hands to its argument (at least `top`, all different), digit by digit:
-// the keys that share the digits so far are counted by the next one. Digits that all keys of `T` scores and of indices
+// the keys that share the digits so far are counted by the next one. A warp's lanes hand theirs over together, a lane
+// without one with `here` false. Digits that all keys of `T` scores and of indices
 // below `n` share are known: an index's high ones, and those of a 16-bit score's low half as f32, which its sign sets.
 template <class T, int kThreads, class Each>
 __device__ __forceinline__ unsigned long long nth_key(Shared<kThreads>& s, uint32_t top, uint32_t n, Each each) {
@@ -76,10 +77,11 @@ __device__ __forceinline__ unsigned long long nth_key(Shared<kThreads>& s, uint3
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < 256; i += kThreads) s.order[i] = 0;
         __syncthreads();
-        each([&](unsigned long long key) {
-            if (shift != 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
+        each([&](unsigned long long key, bool here) {
+            here = here && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+            const uint32_t d = static_cast<uint32_t>(key >> shift) & 255u, lanes = __ballot_sync(kFull, here);
+            if (!here) return;
             // Equal scores share their digits: one addition for the lanes that are here.
-            const uint32_t d = static_cast<uint32_t>(key >> shift) & 255u, lanes = __activemask();
             int same;
             __match_all_sync(lanes, d, &same);
             if (same == 0)
@@ -120,7 +122,10 @@ __device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t co
     const uint32_t t = threadIdx.x;
     if (count > kRanked) {
         const unsigned long long last = nth_key<T>(s, top, n, [&](auto f) {
-            for (uint32_t i = t; i < count; i += kThreads) f(s.key[i]);
+            for (uint32_t base = 0; base < count; base += kThreads) {
+                const uint32_t i = base + t;
+                f(i < count ? s.key[i] : 0ull, i < count);
+            }
         });
         if (t == 0) s.count = 0;
         __syncthreads();
@@ -152,19 +157,22 @@ __device__ __forceinline__ void rank_candidates(Shared<kThreads>& s, uint32_t co
     }
 }
 
-// Entries [from, to) of the vectors and, for share 0, the scalars outside them, each to `f(score, index)`.
+// Entries [from, to) of the vectors and, for share 0, the scalars outside them, each to `f(score, index, true)`. A warp's
+// lanes call `f` together: one that has no entry left with -inf and false.
 template <class T, int kVec, int kThreads, class F>
 __device__ __forceinline__ void for_share(const Walk<T, kVec>& w, uint32_t from, uint32_t to, bool edges, F f) {
-    for (uint32_t v = from + threadIdx.x; v < to; v += kThreads) {
+    for (uint32_t base = from; base < to; base += kThreads) {
+        const uint32_t v = base + threadIdx.x;
         Pack<T, kVec> p;
-        p.load(w.z + w.at(v));
+        p.masked();
+        if (v < to) p.load(w.z + w.at(v));
         float x[kVec];
         p.values(x);
-        for (int e = 0; e < kVec; ++e) f(x[e], w.at(v) + e);
+        for (int e = 0; e < kVec; ++e) f(x[e], w.at(v) + e, v < to);
     }
     if (edges) {
-        const uint32_t j = w.edge(threadIdx.x);
-        if (threadIdx.x < 2 * kVec && j < w.n) f(to_float(w.z[j]), j);
+        const uint32_t j = threadIdx.x < 2 * kVec ? w.edge(threadIdx.x) : w.n;
+        f(j < w.n ? to_float(w.z[j]) : -CUDART_INF_F, j, j < w.n);
     }
 }
 
@@ -175,15 +183,13 @@ __device__ __noinline__ void select_candidates(Shared<kThreads>& s, const T* z, 
                                                uint32_t top) {
     const Walk<T, kVec> w(z, n);
     auto each = [&](auto f) {
-        for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j) {
-            if (x > -CUDART_INF_F) f(order_key(x, j));
-        });
+        for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t j, bool) { f(order_key(x, j), x > -CUDART_INF_F); });
     };
     const unsigned long long last = nth_key<T>(s, top, n, each);
     if (threadIdx.x == 0) s.keys = 0;
     __syncthreads();
-    each([&](unsigned long long key) {
-        if (key >= last) s.key[take(&s.keys)] = key;
+    each([&](unsigned long long key, bool here) {
+        if (here && key >= last) s.key[take(&s.keys)] = key;
     });
     __syncthreads();
 }
@@ -195,8 +201,9 @@ __device__ __noinline__ Stats far_stats(Shared<kThreads>& s, const T* z, uint32_
                                         float c) {
     const Walk<T, kVec> w(z, n);
     Stats a{-FLT_MAX, 0.0f, 0.0f};
-    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t) { a.m = fmaxf(a.m, x); });
-    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t) {
+    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t, bool) { a.m = fmaxf(a.m, x); });
+    for_share<T, kVec, kThreads>(w, from, to, edges, [&](float x, uint32_t, bool here) {
+        if (!here) return;
         const float y = exponent(x, a.m, c), p = pow2(y);
         a.s += p;
         a.v = __fmaf_rn(p, y, a.v);

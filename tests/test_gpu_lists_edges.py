@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import torch
-from test_gpu_lists import TYPES, backend, check_distill, dense, random_teacher  # noqa: F401
+from test_gpu_lists import TYPES, backend, check_distill, check_log_probs, dense, random_teacher, rows_of  # noqa: F401
 
 from silvic_b200 import TeacherTop
 
@@ -31,3 +31,18 @@ def test_a_warp_s_lanes_share_the_teacher(backend, width, top, rest, type_):  # 
     teacher = TeacherTop(ids, teacher.logits.contiguous(), teacher.log_sum, 1.3)
     for _ in range(3):
         check_distill(scores, teacher, backend.distill(scores, teacher, hessian=True), None, None, type_)
+
+
+@pytest.mark.parametrize("lists,width", [(3, 700), (300, 9001), (5, 40000), (160, 2049)])
+def test_equal_scores_are_counted_by_whole_warps(backend, lists, width):  # noqa: F811
+    """More equal scores than a CTA gathers: the alternatives come from counts of digits, by warps of which some lanes
+    have no entry left."""
+    rng = np.random.RandomState(width)
+    scores = torch.from_numpy(rng.randint(0, 2, (lists, width)).astype(np.float32)).cuda()
+    scores[0] = 1.0
+    scores[1, ::3] = -np.inf
+    some = min(lists, 6)
+    for top in (31, 128):
+        got = backend.log_probs(scores, top=top)
+        check_log_probs(scores[:some], rows_of(scores[:some]), None, top, 1.0,
+                        type(got)(None, got.entropy[:some], got.log_sum[:some], got.top_ids[:some], got.top[:some]))
