@@ -457,7 +457,8 @@ int sb2_log_probs(sb2_backend* b, const sb2_lists* lists, double temperature, co
 
 /* The distillation loss of every list and its derivatives. With the student's p = softmax(z / T), the teacher's q
  * over its top, r = 1 - sum q the teacher's rest (0 without log_sum_dev, or where the student has no mass outside the
- * top), P the student's mass outside the top and Q = sum q + r:
+ * top: every entry there masked, or about 744 T and more below the rest, where p is 0 in 64 bits too), P the student's
+ * mass outside the top, which may be far below what f32 holds, and Q = sum q + r:
  *   loss_dev [num_lists]  weight * (sum q (ln q - ln p) + r (ln r - ln P))
  *   grad_dev              d loss / d z_j = weight / T * (Q p_j - q_j) in the top, weight / T * p_j (Q - r / P) elsewhere
  *   hess_dev              weight / T^2 * Q p_j (1 - p_j), the diagonal of the softmax's own second derivative

@@ -8,7 +8,8 @@
 //            w / T p_j (Q - r / P)          elsewhere
 //   hess_j = w / T^2 Q p_j (1 - p_j)        (the diagonal of the softmax's own second derivative)
 // P is summed over the entries outside the top, not taken as 1 - sum p: a student that has learned its teacher keeps
-// little there. The top's entries are marked in a bitmap, which the sum skips; their gradients are written once the
+// little there. Where that is less than 2^-40, the entries outside go about their own maximum in a pass of their own: f32
+// holds the gradient's r p_j / P however small P is. The top's entries are marked in a bitmap, which the sum skips; their gradients are written once the
 // others are, over what the common formula left there. An entry named twice has its q added in the teacher's order.
 //
 // Lists of at most 512 entries (1024 of a dense matrix) take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
@@ -44,6 +45,12 @@ constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
 constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
 
+// Share of the student's mass outside the top below which that part is taken about its own maximum: terms below 2^-126
+// are 0, and those above are still 2^-86 of it.
+constexpr float kApart = 0x1p-40f;
+// ... and P's binary exponent from which it counts as none, as in 64 bits.
+constexpr float kNoMass = -1074.0f;
+
 constexpr uint32_t kBits = 65536;    // marks of a share: entries past so many share them
 
 // What the derivatives of a list's entries share: with e = exp((z - m) / T) and p = inv_s e, the gradient is slope e
@@ -64,6 +71,9 @@ struct Shared {
     Slopes slopes;                   // what one warp makes of the sums, for the others
     float joined_m, q_scale;
     int32_t empty;
+    int32_t apart;                   // the entries outside the top go about their own maximum
+    float sum, held, cross, r;       // what that takes
+    float rest_m, rest_sum;          // the share's maximum and sum outside the top
     uint32_t edge_bits;              // marks of the scalars outside the vectors
 };
 
@@ -153,12 +163,17 @@ __device__ __forceinline__ void teacher_entry(const DistillArgs& a, uint32_t i, 
     y = id >= 0 ? load_typed(a.t.logits, a.t.type, at) * a.inv_t : -CUDART_INF_F;
 }
 
-// The loss of a list from its parts: sum q (log q - (z - m) / T), sum q, the sums S and S P, and the rest.
-__device__ __forceinline__ float loss_of(float cross, float held, float sum, float outside, float r) {
+// The loss of a list from its parts: sum q (log q - (z - m) / T), sum q, S, log (S P), and the rest.
+__device__ __forceinline__ float loss_of(float cross, float held, float sum, float log_outside, float r) {
     const float log_s = logf(sum);
     float loss = cross + held * log_s;
-    if (r > 0.0f) loss += r * (logf(r) - (logf(outside) - log_s));
+    if (r > 0.0f) loss += r * (logf(r) - (log_outside - log_s));
     return loss;
+}
+
+// Whether a maximum outside the top leaves P a mass: less than 64 bits hold counts as none, as a masked entry's.
+__device__ __forceinline__ bool has_mass(float rest_m, float m, float sum, float c) {
+    return (rest_m - m) * c - log2f(sum) >= kNoMass;
 }
 
 __device__ __forceinline__ Slopes slopes_of(float w, float inv_t, float held, float r, float sum, float outside) {
@@ -169,6 +184,11 @@ __device__ __forceinline__ Slopes slopes_of(float w, float inv_t, float held, fl
     k.slope = r > 0.0f ? (mass * k.inv_s - r / outside) * (w * inv_t) : k.top_slope;
     k.curve = mass * (w * inv_t * inv_t);
     return k;
+}
+
+// Whether what lies outside the top needs its own maximum, for a rest of `r` (k: the slopes without it).
+__device__ __forceinline__ bool rest_is_apart(float r, float sum, float outside, const Slopes& k) {
+    return r > 0.0f && (outside < kApart * sum || fabsf(k.slope) == CUDART_INF_F);
 }
 
 // Marks the teacher's entry `id` where it lies in this share (true). s.again: a mark that was set before.
@@ -252,9 +272,86 @@ __device__ __forceinline__ void share_of(const Walk<T, kVec>& w, uint32_t share,
     }
 }
 
+// What is left of a list once its sums are known and little mass lies outside the top (Shared::apart): the loss and all
+// derivatives, the entries outside the top about their own maximum.
+template <class T, int kVec, int kThreads, bool kCluster>
+__device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const uint32_t* bits, const DistillArgs& a, uint32_t i, uint32_t share,
+                                          uint32_t shares, Maxima most) {
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    uint64_t first;
+    uint32_t n;
+    list_range(a.l, i, first, n);
+    const Walk<T, kVec> w(static_cast<const T*>(a.l.scores) + first, n);
+    uint32_t from, to;
+    share_of<T, kVec, kCluster>(w, share, shares, from, to);
+    const float c = __fmul_rn(kLog2E, a.inv_t), weight = a.weight != nullptr ? a.weight[i] : 1.0f, m = s.joined_m, sum = s.sum;
+    const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
+    auto each = [&](auto f) {
+        for (uint32_t v = from + t; v < to; v += kThreads) {
+            const uint32_t skip = marks_of(s, bits, bits != nullptr, w, from, to, a.t.top, v);
+            Pack<T, kVec> p;
+            float x[kVec];
+            p.load(w.z + w.at(v));
+            p.values(x);
+            for (int e = 0; e < kVec; ++e)
+                if (((skip >> e) & 1u) == 0) f(x[e], w.at(v) + e);
+        }
+        if (edge_at < n && ((s.edge_bits >> t) & 1u) == 0) f(to_float(w.z[edge_at]), edge_at);
+    };
+    float rest_m = -CUDART_INF_F, rest_sum = 0.0f;
+    each([&](float z, uint32_t) { rest_m = fmaxf(rest_m, z); });
+    rest_m = warp_max(rest_m);
+    if (lane == 0) s.warp[0][warp] = rest_m;
+    __syncthreads();
+    rest_m = max_of<kThreads>(s.warp[0]);
+    if constexpr (kCluster) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (t == 0) s.rest_m = rest_m;
+        cluster.sync();
+        rest_m = warp_max(cluster.map_shared_rank(&s, lane & (shares - 1))->rest_m);
+    }
+    const bool some = has_mass(rest_m, m, sum, c);
+    if (some) each([&](float z, uint32_t) { rest_sum += pow2(exponent(z, rest_m, c)); });
+    rest_sum = warp_sum(rest_sum);
+    if (lane == 0) s.warp[1][warp] = rest_sum;
+    __syncthreads();
+    rest_sum = sum_of<kThreads>(s.warp[1]);
+    if constexpr (kCluster) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (t == 0) s.rest_sum = rest_sum;
+        cluster.sync();
+        const float other = cluster.map_shared_rank(&s, lane & (shares - 1))->rest_sum;
+        rest_sum = warp_sum(lane < shares ? other : 0.0f);
+    }
+    const float r = some ? s.r : 0.0f;
+    if (t == 0 && share == 0 && a.loss != nullptr)
+        a.loss[i] = weight * loss_of(s.cross, s.held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
+    if (a.grad == nullptr && a.hess == nullptr) return most;
+    const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
+    const float mass = s.held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
+    auto put_one = [&](float z, uint32_t j, float less) {
+        const float p = pow2(exponent(z, m, c)) * inv_s;
+        put<T>(a, out + j, first + j, (mass * p - less) * scale, mass * scale * a.inv_t * p * (1.0f - p), true, most);
+    };
+    each([&](float z, uint32_t j) { put_one(z, j, some ? pull * pow2(exponent(z, rest_m, c)) : 0.0f); });
+    if (t < a.t.top && s.id[t] >= 0) {  // the top's own in this share, the first that names an index with all their q
+        const uint32_t id = static_cast<uint32_t>(s.id[t]);
+        bool leads = id < w.head || id >= w.tail() ? share == 0 : (id - w.head) / kVec >= from && (id - w.head) / kVec < to;
+        for (uint32_t k = 0; k < t && leads; ++k) leads = s.id[k] != s.id[t];
+        if (leads) {
+            float q = 0.0f;
+            for (uint32_t k = t; k < a.t.top; ++k)
+                if (s.id[k] == s.id[t]) q += s.q[k];
+            put_one(to_float(w.z[id]), id, q);
+        }
+    }
+    return most;
+}
+
 // One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1). `data` holds `slots` vectors:
 // where the share is no longer, it stays there, each vector in a slot of the thread that reads it. A slot is free once
-// its gradient is written, so list `next` (no list from a.l.lists on) follows through the same slots at once.
+// its gradient is written, so list `next` (no list from a.l.lists on) follows through the same slots at once. `bits` may be
+// null: the teacher's ids are then looked through for each vector.
 template <class T, int kVec, int kThreads, bool kCluster>
 __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>* data, uint32_t slots, uint32_t* bits,
                                              const DistillArgs& a, uint32_t i, uint32_t next, Ahead& ahead, uint32_t share,
@@ -269,7 +366,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     share_of<T, kVec, kCluster>(w, share, shares, from, to);
     const float c = __fmul_rn(kLog2E, a.inv_t);
     const bool rest = a.t.log_sum != nullptr;
-    const bool held_here = kVec == 1 || to - from <= slots;
+    const bool held_here = kVec == 1 || to - from <= slots, room = bits != nullptr;
     const float log_sum = rest ? a.t.log_sum[i] : 0.0f, weight = a.weight != nullptr ? a.weight[i] : 1.0f;
     // The scores, on their way to the thread's own slots.
     if (kVec > 1 && held_here && !ahead.flying) {
@@ -294,11 +391,11 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     }
     ahead.flying = false;
     if (t < kMaxTop) s.id[t] = id;
-    const uint32_t words = held_here ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
+    const uint32_t words = room ? (min(kBits, (to - from) * kVec) + 31) / 32 : 0;
     for (uint32_t k = t; k < words; k += kThreads) bits[k] = 0;
     if (t == 0) s.edge_bits = s.again = 0;
     __syncthreads();
-    const bool mine = mark_entry(s, bits, held_here, w, from, to, share, id);
+    const bool mine = mark_entry(s, bits, room, w, from, to, share, id);
     // Vector `v` of the share; a run between boundaries, entry by entry, is read from its place each time.
     auto get = [&](uint32_t v, float(&x)[kVec]) {
         if constexpr (kVec == 1)
@@ -306,7 +403,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         else
             data[v].values(x);
     };
-    auto marked = [&](uint32_t v) { return marks_of(s, bits, held_here, w, from, to, a.t.top, v); };
+    auto marked = [&](uint32_t v) { return marks_of(s, bits, room, w, from, to, a.t.top, v); };
     // The maxima of the scores and of the teacher's.
     float m = fmaxf(edge, zt);  // with the top's scores, so that no share's reference lies far below them
     if constexpr (kVec == 1) {
@@ -445,10 +542,12 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
             cross = cross * q_scale - logf(held);
             held = 1.0f;
         }
-        const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+        const float r = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
         const bool none = sum == 0.0f || !taught;
         // What the derivatives outside the top share, and what the same formula gives in it.
         Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
+        const bool apart = !none && rest_is_apart(r, sum, outside, k);
+        if (apart) k = slopes_of(weight, a.inv_t, held, 0.0f, sum, outside);
         R = __fmul_rn(m, c);
         if (fabsf(R) < kFar && held_here) {  // the terms are about R
             const float f = pow2(-__fmaf_rn(m, c, -R));
@@ -461,10 +560,23 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
             s.joined_m = m;
             s.q_scale = q_scale;
             s.empty = none;
-            if (share == 0 && a.loss != nullptr) a.loss[i] = none ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+            s.apart = apart;
+            if (apart) {
+                s.sum = sum;
+                s.held = held;
+                s.cross = cross;
+                s.r = r;
+            } else if (share == 0 && a.loss != nullptr) {
+                a.loss[i] = none ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), r);
+            }
         }
     }
     __syncthreads();
+    if (s.apart != 0) {  // (every share of a cluster joins the same sums)
+        most = rest_apart<T, kVec, kThreads, kCluster>(s, bits, a, i, share, shares, most);
+        if constexpr (kCluster) cg::this_cluster().sync();  // the shares' memory is read
+        return;
+    }
     if constexpr (kCluster) cg::this_cluster().barrier_arrive();  // the shares' memory is read
     if (a.grad == nullptr && a.hess == nullptr) {
         if constexpr (kCluster) cg::this_cluster().barrier_wait();
@@ -589,7 +701,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
 }
 
 // The loss alone of one dense list: its sums are taken while it is read, about the maximum of the first batch (moved
-// where later entries lie far above it). False: far scores, which distill_list() takes.
+// where later entries lie far above it). False: far scores, or little mass outside the top: distill_list() takes it.
 template <class T, int kVec, int kThreads, bool kCluster>
 __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, const DistillArgs& a, uint32_t i, uint32_t share,
                                           uint32_t shares) {
@@ -729,22 +841,21 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
         top_sum = warp_sum(lane < shares ? other_top * f : 0.0f);
         cluster.sync();  // the shares' memory is read
     }
-    if (far) return false;
+    const float sum = outside + top_sum, rest_q = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+    if (far || (rest_q > 0.0f && sum != 0.0f && taught && outside < kApart * sum)) return false;
     if (t == 0 && share == 0) {
         cross += held * ((all - m) * a.inv_t);
         if (!rest && held != 0.0f) {
             cross = cross / held - logf(held);
             held = 1.0f;
         }
-        const float sum = outside + top_sum;
-        const float rest_q = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
-        a.loss[i] = sum == 0.0f || !taught ? 0.0f : weight * loss_of(cross, held, sum, outside, rest_q);
+        a.loss[i] = sum == 0.0f || !taught ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), rest_q);
     }
     return true;
 }
 
 template <class T, int kVec, int kThreads, bool kCluster>
-__global__ void __launch_bounds__(kThreads) distill_loss_kernel(DistillArgs a, uint32_t shares) {
+__global__ void __launch_bounds__(kThreads) distill_loss_kernel(const __grid_constant__ DistillArgs a, uint32_t shares) {
     __shared__ Shared<kThreads> s;
     extern __shared__ __align__(16) unsigned char held[];
     uint32_t* bits = reinterpret_cast<uint32_t*>(held);
@@ -758,13 +869,14 @@ __global__ void __launch_bounds__(kThreads) distill_loss_kernel(DistillArgs a, u
 }
 
 template <class T, int kVec, int kThreads, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(DistillArgs a, uint32_t shares, uint32_t slots) {
+__global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(const __grid_constant__ DistillArgs a, uint32_t shares, uint32_t slots) {
     if (a.stopped != nullptr && *a.stopped) return;
     extern __shared__ __align__(16) unsigned char held[];
     __shared__ Shared<kThreads> s;
     Maxima most;
     Pack<T, kVec>* data = reinterpret_cast<Pack<T, kVec>*>(held);
     uint32_t* bits = reinterpret_cast<uint32_t*>(held + ((slots * sizeof(Pack<T, kVec>) + 15) & ~static_cast<size_t>(15)));
+    if (kVec > 1 && slots == 0) bits = nullptr;  // no shared memory at all
     const uint32_t shift = kCluster ? __ffs(shares) - 1 : 0, step = gridDim.x >> shift;
     Ahead ahead;
     for (uint32_t i = blockIdx.x >> shift; i < a.l.lists; i += step) {
@@ -780,6 +892,49 @@ struct WarpShared {
     int32_t id[kMaxTop];
     float q[kMaxTop];
 };
+
+// rest_apart() of a warp's list (`cross`: a lane's part).
+template <class T>
+__device__ __noinline__ Maxima warp_rest_apart(const WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n, float m,
+                                               float sum, float held, float cross, Maxima most) {
+    const uint32_t lane = threadIdx.x & 31;
+    const T* z = static_cast<const T*>(a.l.scores) + first;
+    const float c = __fmul_rn(kLog2E, a.inv_t), weight = a.weight != nullptr ? a.weight[i] : 1.0f;
+    auto each = [&](auto f) {
+        for (uint32_t j = lane; j < n; j += 32)
+            if (((s.bits[j / 32] >> lane) & 1u) == 0) f(to_float(z[j]), j);
+    };
+    float rest_m = -CUDART_INF_F, rest_sum = 0.0f;
+    each([&](float x, uint32_t) { rest_m = fmaxf(rest_m, x); });
+    rest_m = warp_max(rest_m);
+    const bool some = has_mass(rest_m, m, sum, c);
+    if (some) each([&](float x, uint32_t) { rest_sum += pow2(exponent(x, rest_m, c)); });
+    rest_sum = warp_sum(rest_sum);
+    const float r = some ? 1.0f - held : 0.0f;
+    cross = warp_sum(cross);
+    if (lane == 0 && a.loss != nullptr)
+        a.loss[i] = weight * loss_of(cross, held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
+    if (a.grad == nullptr && a.hess == nullptr) return most;
+    const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
+    const float mass = held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
+    auto put_one = [&](float x, uint32_t j, float less) {
+        const float p = pow2(exponent(x, m, c)) * inv_s;
+        put<T>(a, out + j, first + j, (mass * p - less) * scale, mass * scale * a.inv_t * p * (1.0f - p), true, most);
+    };
+    each([&](float x, uint32_t j) { put_one(x, j, some ? pull * pow2(exponent(x, rest_m, c)) : 0.0f); });
+    __syncwarp();  // the lanes' q
+    for (uint32_t k = lane; k < a.t.top; k += 32) {
+        const int32_t id = s.id[k];
+        bool leads = id >= 0;
+        for (uint32_t e = 0; e < k && leads; ++e) leads = s.id[e] != id;
+        if (!leads) continue;
+        float q = 0.0f;
+        for (uint32_t e = k; e < a.t.top; ++e)
+            if (s.id[e] == id) q += s.q[e];
+        put_one(to_float(z[id]), static_cast<uint32_t>(id), q);
+    }
+    return most;
+}
 
 // A list of at most 32 kItems entries by one warp, in registers; kTop of the teacher's entries a lane.
 template <class T, int kItems, int kTop>
@@ -870,15 +1025,19 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         if (u * 32 + lane < a.t.top) s.q[u * 32 + lane] = q[u];
     }
     held = warp_sum(held);
-    const float r = rest && outside > 0.0f ? fmaxf(1.0f - held, 0.0f) : 0.0f;
+    const float r = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
     const bool empty = sum == 0.0f || !taught;
     const float weight = a.weight != nullptr ? a.weight[i] : 1.0f;
+    const Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
+    if (!empty && rest_is_apart(r, sum, outside, k)) {
+        most = warp_rest_apart<T>(s, a, i, first, n, m, sum, held, cross, most);
+        return;
+    }
     if (a.loss != nullptr) {
         cross = warp_sum(cross);
-        if (lane == 0) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, outside, r);
+        if (lane == 0) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), r);
     }
     if (a.grad == nullptr && a.hess == nullptr) return;
-    const Slopes k = slopes_of(weight, a.inv_t, held, r, sum, outside);
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
@@ -906,7 +1065,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
 // `per` lists a CTA (8 at most), a warp each of at most 32 kMost entries; a longer one among them by the whole CTA. So what a list gives depends on
 // its own length alone.
 template <class T, int kTop, int kMost>
-__global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4) distill_warps_kernel(DistillArgs a, uint32_t per) {
+__global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4) distill_warps_kernel(const __grid_constant__ DistillArgs a, uint32_t per) {
     constexpr uint32_t kEntries = 32 * kMost;
     if (a.stopped != nullptr && *a.stopped) return;
     __shared__ WarpShared warps[kWarpThreads / 32];

@@ -3,12 +3,14 @@ near what f32 holds; against the definitions in 64 bits (lists_reference.py)."""
 
 from __future__ import annotations
 
+import lists_reference as ref
 import numpy as np
 import pytest
 import torch
+from synth import ranking_binned
 from test_gpu_lists import TYPES, backend, check_distill, check_log_probs, dense, random_teacher, rows_of  # noqa: F401
 
-from silvic_b200 import TeacherTop
+from silvic_b200 import B200Backend, TeacherTop, _abi
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +48,134 @@ def test_equal_scores_are_counted_by_whole_warps(backend, lists, width):  # noqa
         got = backend.log_probs(scores, top=top)
         check_log_probs(scores[:some], rows_of(scores[:some]), None, top, 1.0,
                         type(got)(None, got.entropy[:some], got.log_sum[:some], got.top_ids[:some], got.top[:some]))
+
+
+# ---- the rest of a confident student -------------------------------------------------------------------------------
+
+
+def check_rest(z, ids, logits, t, log_sum, w, loss, grad, hess, type_):
+    """A list whose mass P outside the top is small, against the definition. p is off by 4 slack(n) and 4 U x of itself
+    (x its distance from the maximum over T: four roundings of the exponent), p / P alike about the maximum outside the
+    top, the teacher's sums by (k + 32 + 4 arg) U, and r = 1 - sum q by as much of 1. An exponential below 2^-126 of its
+    maximum's is 0. Then half a step of the type."""
+    with np.errstate(over="ignore"):  # r / P times p, at the top's own
+        want = ref.distill(z, ids, logits, t, log_sum, w)
+    q, inside, held, _ = ref.teach(len(z), ids, logits, t, log_sum)
+    p, lp, _ = ref.softmax(z, t)
+    rest_p = p[~inside].sum()
+    live = [abs(float(v)) / t for i, v in zip(ids, logits) if 0 <= int(i) < len(z)]
+    own = (len(ids) + 32 + 4 * (max(live, default=0.0) + abs(log_sum))) * ref.U
+    relative = 4 * ref.slack(len(z)) + own
+    assert np.isfinite(loss) and abs(loss - want["loss"]) <= 2 * relative * want["terms"] + 1e-37, (loss, want["loss"])
+    step, least = {"f32": (2.0 ** -24, 2.0 ** -150), "bf16": (2.0 ** -8, 2.0 ** -134), "f16": (2.0 ** -11, 2.0 ** -25)}[type_]
+    fine = np.isfinite(z)
+    x = np.where(fine, -np.where(fine, lp, 0.0), 0.0)
+    mass, scale, tiny = held, w / t, 2.0 ** -125 * w / t * (1 + held)
+    of_rest, x_rest = np.zeros(len(z)), np.zeros(len(z))
+    if rest_p > 0 and held < 1:
+        mass = 1.0
+        of_rest = np.where(inside, 0.0, p / rest_p)
+        x_rest = np.where(fine & ~inside, (z[~inside].max() - np.where(fine, z, 0.0)) / t, 0.0)
+    if grad is not None:
+        tol = scale * (mass * p * (relative + 4 * ref.U * x) + q * relative + of_rest * (own + relative + 4 * ref.U * x_rest))
+        tol = tol + step * 1.001 * np.abs(want["grad"]) + least + tiny
+        bad = ~(np.abs(grad - want["grad"]) <= tol)
+        assert not bad.any(), (np.nonzero(bad)[0][:5], grad[bad][:5], want["grad"][bad][:5], tol[bad][:5])
+    if hess is not None:
+        tol = scale / t * p * ((relative + 4 * ref.U * x) * (1 + p) + 4 * ref.U) * max(mass, 1.0)
+        tol = tol + step * 1.001 * np.abs(want["hess"]) + least + tiny / t
+        bad = ~(np.abs(hess - want["hess"]) <= tol)
+        assert not bad.any(), (np.nonzero(bad)[0][:5], hess[bad][:5], want["hess"][bad][:5], tol[bad][:5])
+
+
+GAPS = [80.0, 86.0, 90.0, 300.0, 700.0, 20.0, 30.0, 60.0]
+
+
+def confident(rng, n, t, i, top, type_):
+    """Scores of n entries and the top's ids: the others lie GAPS nats below the top, some of them masked; of every
+    eleventh list all of them, of the next all by the type's lowest value (no mass in 64 bits either)."""
+    ids = rng.choice(n, min(top, n), replace=False)
+    z = rng.randn(n) * 2 * t
+    z[ids] += (GAPS[i % len(GAPS)] + 8.0) * t
+    outside = np.setdiff1d(np.arange(n), ids)
+    if len(outside) > 1:
+        z[outside[1:][rng.rand(len(outside) - 1) < 0.3]] = -np.inf
+    if i % 11 == 9:
+        z[outside] = -np.inf
+    if i % 11 == 10:
+        z[outside] = torch.finfo(TYPES[type_]).min
+    return z, ids
+
+
+@pytest.mark.parametrize("weight", [1.0, 65536.0])
+@pytest.mark.parametrize("t", [1.0, 0.1, 0.01])
+@pytest.mark.parametrize("type_,sizes", [
+    ("f32", [300] * 12), ("bf16", [513] * 11), ("f16", [1000] * 12), ("f32", [5000] * 5), ("bf16", [5001] * 300),
+    ("bf16", [40001] * 3), ("f32", [20011] * 300), ("f16", [70001] * 160), ("f32", [300007] * 2), ("f32", [500003] * 2),
+    ("f32", [5, 300, 700, 5000, 0, 130, 90000, 2000]), ("f32", [7, 40, 3, 600] * 6), ("f16", [900, 3000, 200])])
+def test_the_rest_of_a_confident_student(backend, type_, sizes, t, weight):  # noqa: F811
+    rng = np.random.RandomState(len(sizes) + sizes[0])
+    if type_ == "f16":
+        weight = min(weight, 4.0)  # gradients of weight / T
+    few = min(len(sizes), 12)
+    uneven = len(set(sizes)) > 1
+    top = 6
+    made = [confident(rng, n, t, i, top, type_) if n else (np.zeros(0), np.zeros(0, int)) for i, n in enumerate(sizes[:few])]
+    ids = np.full((len(sizes), top), -1, np.int32)
+    for i in range(len(sizes)):
+        some = made[i % few][1]
+        ids[i, : len(some)] = some
+    rows = [torch.from_numpy(made[i % few][0]).to(TYPES[type_]) for i in range(len(sizes))]
+    boundaries = None
+    if uneven:
+        scores = torch.cat(rows).cuda()
+        bounds = np.concatenate([[0], np.cumsum(sizes)])
+        boundaries = torch.from_numpy(bounds.astype(np.int32)).cuda()
+    else:
+        scores = torch.stack(rows).cuda()
+    logits = torch.from_numpy(rng.randn(len(sizes), top) * 2 * t).float()
+    x = torch.where(torch.from_numpy(ids) >= 0, logits.double() / t, -np.inf)
+    log_sum = torch.logsumexp(x, 1) + 0.3
+    log_sum = torch.where(torch.isfinite(log_sum), log_sum, 0.0).float()
+    teacher = TeacherTop(torch.from_numpy(ids).cuda(), logits.cuda(), log_sum.cuda(), t)
+    w = torch.full((len(sizes),), weight, device="cuda")
+    both = backend.distill(scores, teacher, boundaries=boundaries, weight=w, hessian=True)
+    alone = backend.distill(scores, teacher, boundaries=boundaries, weight=w, gradient=False)
+    grad_only = backend.distill(scores, teacher, boundaries=boundaries, weight=w)
+    for got in (both, alone, grad_only):
+        parts = [None if v is None else v.double().cpu().numpy() for v in (got.loss, got.gradient, got.hessian)]
+        for i in range(few):
+            z = rows[i].double().numpy()
+            at = slice(bounds[i], bounds[i + 1]) if uneven else i
+            check_rest(z, ids[i], logits[i].numpy(), t, float(log_sum[i]), weight, parts[0][i],
+                       None if parts[1] is None else parts[1][at], None if parts[2] is None else parts[2][at], type_)
+
+
+def test_the_rest_of_a_confident_student_in_training(device):
+    """Scores 90 and 0 by a tree, the teacher's top the high rows: the gradients of the low ones, and their maximum."""
+    data = ranking_binned(2_000, [31] * 3, seed=4, mean_query=40.0)
+    bounds = data.query_boundaries.astype(np.int64)
+    rng = np.random.RandomState(1)
+    node = _abi.DeviceNode()
+    node.split.left_bins[0] = 0x3FF  # of group 0's column 0
+    node.left, node.right = ~0, ~1
+    with B200Backend(device) as b:
+        b.load(data, "distill")
+        b.add_tree([node], [0.0, 90.0])
+        scores = b.scores()
+        assert set(np.unique(scores)) == {0.0, 90.0}
+        ids = np.full((len(bounds) - 1, 100), -1, np.int32)
+        for i, (a, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+            high = np.nonzero(scores[a:e] == 90.0)[0]
+            ids[i, : len(high)] = high
+        logits = rng.randn(*ids.shape).astype(np.float32)
+        total = np.log(np.where(ids >= 0, np.exp(logits.astype(np.float64)), 0.0).sum(1) + 1e-300)
+        log_sum = np.where(total > -100, total + 0.4, 0.0).astype(np.float32)
+        b.set_teacher(TeacherTop(ids, logits, log_sum))
+        most_g, most_h = b.compute_gradients()
+        g, h = b.read_gradients()
+    assert most_g == np.abs(g).max() and most_h == np.abs(h).max() and np.isfinite([most_g, most_h]).all()
+    for i, (a, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        if (ids[i] >= 0).any():
+            loss = ref.distill(scores[a:e].astype(np.float64), ids[i], logits[i], 1.0, float(log_sum[i]))["loss"]
+            check_rest(scores[a:e].astype(np.float64), ids[i], logits[i], 1.0, float(log_sum[i]), 1.0, loss, g[a:e], h[a:e], "f32")
