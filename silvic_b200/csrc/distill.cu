@@ -94,6 +94,9 @@ __device__ __forceinline__ float max_of(const float (&part)[kThreads / 32]) {
     return v;
 }
 
+// The hessian diagonal of an entry: a p that its roundings carry past 1 makes it 0, never negative.
+__device__ __forceinline__ float hessian_of(float curve, float p) { return curve * p * fmaxf(1.0f - p, 0.0f); }
+
 // Writes an entry's derivatives; the objective's row weight and maxima come in here.
 struct Maxima {
     float g = 0.0f, h = 0.0f;
@@ -331,7 +334,7 @@ __device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const uint32_t* b
     const float mass = s.held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
     auto put_one = [&](float z, uint32_t j, float less) {
         const float p = pow2(exponent(z, m, c)) * inv_s;
-        put<T>(a, out + j, first + j, (mass * p - less) * scale, mass * scale * a.inv_t * p * (1.0f - p), true, most);
+        put<T>(a, out + j, first + j, (mass * p - less) * scale, hessian_of(mass * scale * a.inv_t, p), true, most);
     };
     each([&](float z, uint32_t j) { put_one(z, j, some ? pull * pow2(exponent(z, rest_m, c)) : 0.0f); });
     if (t < a.t.top && s.id[t] >= 0) {  // the top's own in this share, the first that names an index with all their q
@@ -592,7 +595,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
     auto put_one = [&](float z, uint32_t j, bool counts) {
         const float e = empty ? 0.0f : term(z), q_j = e * k.inv_s;
-        put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * e, empty ? 0.0f : k.curve * q_j * (1.0f - q_j), counts, most);
+        put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * e, empty ? 0.0f : hessian_of(k.curve, q_j), counts, most);
     };
     // The next list's scores follow into each slot as its gradient is written.
     const T* next_z = nullptr;
@@ -629,7 +632,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                 get(v, x);
                 const float e = pow2(__fmaf_rn(x[0], c, -R)), p_j = e * k.inv_s;
                 if (grad != nullptr) grad[v] = from_float<T>(k.slope * e);
-                if (hess != nullptr) hess[v] = from_float<T>(k.curve * p_j * (1.0f - p_j));
+                if (hess != nullptr) hess[v] = from_float<T>(hessian_of(k.curve, p_j));
             }
         } else if (kVec > 1 && aligned && grad != nullptr && hess == nullptr) {
 #pragma unroll kUnroll
@@ -657,7 +660,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                 for (int e = 0; e < kVec; ++e) {
                     const float z = pow2(__fmaf_rn(x[e], c, -R)), p_j = z * k.inv_s;
                     g[e] = k.slope * z;
-                    h[e] = k.curve * p_j * (1.0f - p_j);
+                    h[e] = hessian_of(k.curve, p_j);
                 }
                 if (kVec > 1 && aligned) {
                     if constexpr (kVec > 1) {
@@ -695,7 +698,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                 if (s.id[x] == id) taught_q += s.q[x] * q_scale;
         }
         const float e = term(zt), p_j = e * k.inv_s;
-        put<T>(a, out + id, first + id, k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p_j * (1.0f - p_j), true, most);
+        put<T>(a, out + id, first + id, k.top_slope * e - taught_q * (weight * a.inv_t), hessian_of(k.curve, p_j), true, most);
     }
     if constexpr (kCluster) cg::this_cluster().barrier_wait();
 }
@@ -919,7 +922,7 @@ __device__ __noinline__ Maxima warp_rest_apart(const WarpShared& s, const Distil
     const float mass = held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
     auto put_one = [&](float x, uint32_t j, float less) {
         const float p = pow2(exponent(x, m, c)) * inv_s;
-        put<T>(a, out + j, first + j, (mass * p - less) * scale, mass * scale * a.inv_t * p * (1.0f - p), true, most);
+        put<T>(a, out + j, first + j, (mass * p - less) * scale, hessian_of(mass * scale * a.inv_t, p), true, most);
     };
     each([&](float x, uint32_t j) { put_one(x, j, some ? pull * pow2(exponent(x, rest_m, c)) : 0.0f); });
     __syncwarp();  // the lanes' q
@@ -1044,7 +1047,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         const uint32_t j = u * 32 + lane;
         const float p = x[u] * k.inv_s;
         if (j < n)
-            put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * x[u], empty ? 0.0f : k.curve * p * (1.0f - p),
+            put<T>(a, out + j, first + j, empty ? 0.0f : k.slope * x[u], empty ? 0.0f : hessian_of(k.curve, p),
                    ((marks >> u) & 1u) == 0, most);
     }
     __syncwarp();  // the top's own go over them
@@ -1058,7 +1061,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
                 if (s.id[e] == id[u]) taught_q += s.q[e];
         }
         const float e = pow2(exponent(zt[u], m, c)), p = e * k.inv_s;
-        put<T>(a, out + id[u], first + id[u], k.top_slope * e - taught_q * (weight * a.inv_t), k.curve * p * (1.0f - p), true, most);
+        put<T>(a, out + id[u], first + id[u], k.top_slope * e - taught_q * (weight * a.inv_t), hessian_of(k.curve, p), true, most);
     }
 }
 

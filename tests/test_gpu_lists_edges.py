@@ -179,3 +179,27 @@ def test_the_rest_of_a_confident_student_in_training(device):
         if (ids[i] >= 0).any():
             loss = ref.distill(scores[a:e].astype(np.float64), ids[i], logits[i], 1.0, float(log_sum[i]))["loss"]
             check_rest(scores[a:e].astype(np.float64), ids[i], logits[i], 1.0, float(log_sum[i]), 1.0, loss, g[a:e], h[a:e], "f32")
+
+
+# ---- the hessian's sign --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("lists,width,uneven", [(400, 600, True), (400, 900, False), (300, 1500, True), (300, 5000, False),
+                                                (3, 40001, False)])
+def test_the_hessian_is_never_negative(backend, lists, width, uneven, rest):  # noqa: F811
+    """One entry with nearly all of the mass, whose p rounds to 1 or past it."""
+    rng = np.random.RandomState(width)
+    z = rng.randn(lists, width) * 3 + rng.randn(lists, 1) * 40
+    ids = rng.randint(0, width, (lists, 3)).astype(np.int32)
+    z[np.arange(lists), ids[:, 0]] += 20 + rng.rand(lists) * 60
+    scores = torch.from_numpy(z).float().cuda()
+    boundaries = None
+    if uneven:
+        scores = scores.flatten()
+        boundaries = torch.arange(0, lists * width + 1, width, dtype=torch.int32, device="cuda")
+    log_sum = torch.full((lists,), 3.0, device="cuda") if rest else None
+    for t in (1.0, 0.3):
+        teacher = TeacherTop(torch.from_numpy(ids).cuda(), torch.from_numpy(rng.randn(lists, 3)).float().cuda(), log_sum, t)
+        got = backend.distill(scores, teacher, boundaries=boundaries, hessian=True)
+        assert (got.hessian >= 0).all() and (got.hessian > 0).any()
