@@ -533,7 +533,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
             const float all = warp_max(other_m), f = pow2(exponent(other_m, all, c));
             outside = warp_sum(lane < shares ? other_outside * f : 0.0f);
             top_sum = warp_sum(lane < shares ? other_top * f : 0.0f);
-            cross += held * ((all - m) * a.inv_t);
+            if (held != 0.0f) cross += held * ((all - m) * a.inv_t);  // (a masked share's m is so low that this may be 0 times inf)
             m = all;
         }
     }
@@ -847,7 +847,7 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
     const float sum = outside + top_sum, rest_q = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
     if (far || (rest_q > 0.0f && sum != 0.0f && taught && outside < kApart * sum)) return false;
     if (t == 0 && share == 0) {
-        cross += held * ((all - m) * a.inv_t);
+        if (held != 0.0f) cross += held * ((all - m) * a.inv_t);  // (a masked first batch's m is so low that this may be 0 times inf)
         if (!rest && held != 0.0f) {
             cross = cross / held - logf(held);
             held = 1.0f;

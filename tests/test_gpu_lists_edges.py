@@ -203,3 +203,25 @@ def test_the_hessian_is_never_negative(backend, lists, width, uneven, rest):  # 
         teacher = TeacherTop(torch.from_numpy(ids).cuda(), torch.from_numpy(rng.randn(lists, 3)).float().cuda(), log_sum, t)
         got = backend.distill(scores, teacher, boundaries=boundaries, hessian=True)
         assert (got.hessian >= 0).all() and (got.hessian > 0).any()
+
+
+# ---- a teacher without mass on masked entries ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rest,logit", [(False, -np.inf), (True, -np.inf), (True, -400.0)])
+@pytest.mark.parametrize("lists,width", [(3, 40001), (300, 40001), (300, 5000), (4, 700)])
+def test_a_teacher_without_mass_on_masked_entries(backend, lists, width, rest, logit):  # noqa: F811
+    """The first nine tenths of each list are masked, the whole top among them, and the teacher gives that nothing: the
+    loss is the rest's alone (0 without one)."""
+    rng = np.random.RandomState(width)
+    z = rng.randn(lists, width) * 2
+    z[:, : width * 9 // 10] = -np.inf
+    scores = torch.from_numpy(z).float().cuda()
+    ids = torch.from_numpy(rng.randint(0, width * 9 // 10, (lists, 4)).astype(np.int32)).cuda()
+    log_sum = torch.full((lists,), 2.0, device="cuda") if rest else None
+    teacher = TeacherTop(ids, torch.full((lists, 4), logit, device="cuda"), log_sum, 0.5)
+    for gradient in (False, True):
+        got = backend.distill(scores, teacher, gradient=gradient, hessian=gradient)
+        assert torch.isfinite(got.loss).all()
+        cut = type(got)(got.loss[:4], got.gradient[:4] if gradient else None, got.hessian[:4] if gradient else None)
+        check_distill(scores[:4], TeacherTop(ids[:4], teacher.logits[:4], None if log_sum is None else log_sum[:4], 0.5), cut)
