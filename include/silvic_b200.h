@@ -267,7 +267,8 @@ int sb2_last_error(const sb2_backend* b, char* buf, size_t len);
 int sb2_name(const sb2_backend* b, char* buf, size_t len);
 
 /* Backend::load: copies the training set to the device and lays it out in 32-feature tiles. Numerical and
- * categorical features alike (the split search scans each by its kind). */
+ * categorical features alike (the split search scans each by its kind). A load that fails over its dataset's contents
+ * leaves the handle without one. */
 int sb2_load(sb2_backend* b, const sb2_dataset* train, const sb2_objective* objective);
 /* Backend::init_scores (dataset 0, the training set) */
 int sb2_init_scores(sb2_backend* b, int dataset, double value);

@@ -642,8 +642,10 @@ int sb2_load(sb2_backend* b, const sb2_dataset* train, const sb2_objective* obje
     if (objective->kind != SB2_REGRESSION && objective->kind != SB2_BINARY && objective->kind != SB2_LAMBDARANK &&
         objective->kind != SB2_DISTILL)
         return b->fail(SB2_EUNSUPPORTED, "objective " + std::to_string(objective->kind) + " has no device gradients");
+    b->loaded = false;  // what follows replaces the last dataset part by part; a load that fails leaves none
     b->ranking = RankArgs{};
     b->teacher = TeacherArgs{};
+    b->queries.clear();
     if (objective->kind == SB2_LAMBDARANK) SB2_TRY(load_ranking(b, train, objective));
     if (objective->kind == SB2_DISTILL) SB2_TRY(load_distillation(b, train));
     const uint32_t F = train->num_features;

@@ -10,7 +10,7 @@ import torch
 from synth import ranking_binned
 from test_gpu_lists import TYPES, backend, check_distill, check_log_probs, dense, random_teacher, rows_of  # noqa: F401
 
-from silvic_b200 import B200Backend, TeacherTop, _abi
+from silvic_b200 import B200Backend, SilvicError, TeacherTop, _abi, params_from_dict
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +225,32 @@ def test_a_teacher_without_mass_on_masked_entries(backend, lists, width, rest, l
         assert torch.isfinite(got.loss).all()
         cut = type(got)(got.loss[:4], got.gradient[:4] if gradient else None, got.hessian[:4] if gradient else None)
         check_distill(scores[:4], TeacherTop(ids[:4], teacher.logits[:4], None if log_sum is None else log_sum[:4], 0.5), cut)
+
+
+# ---- a handle whose second load fails ------------------------------------------------------------------------------
+
+
+def test_a_failed_load_leaves_no_dataset_behind(device):
+    """The second dataset's queries are taken before its features are refused: nothing works on a mixture of the two."""
+    data = ranking_binned(3_000, [31] * 3, seed=2, mean_query=10.0)
+    queries = len(data.query_boundaries) - 1
+    teacher = TeacherTop(np.zeros((queries, 1), np.int32), np.zeros((queries, 1), np.float32))
+    p = params_from_dict({"objective": "distill", "num_leaves": 4, "num_iterations": 1})
+    for objective in ("lambdarank", "distill"):
+        bad = ranking_binned(500, [31] * 3, seed=3, mean_query=40.0)
+        bad.features[1].upper_bounds = bad.features[1].upper_bounds[:2]
+        with B200Backend(device) as b:
+            b.load(data, "distill", params=p)
+            b.set_teacher(teacher)
+            b.compute_gradients()
+            want = b.read_gradients()
+            with pytest.raises(SilvicError, match="upper bounds"):
+                b.load(bad, objective)
+            for call in (lambda: b.set_teacher(teacher), b.compute_gradients, lambda: b.train(p, 0.0), b.scores):
+                with pytest.raises(SilvicError, match="before load"):
+                    call()
+            b.load(data, "distill", params=p)
+            b.set_teacher(teacher)
+            b.compute_gradients()
+            for x, y in zip(want, b.read_gradients()):
+                assert np.array_equal(x, y)
