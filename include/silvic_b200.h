@@ -475,7 +475,9 @@ int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* tea
  * before gradients or training: num_queries rows of `top` ids (a row's index within its query, -1: padding) and
  * logits in host memory, log_sum NULL or num_queries values, as in sb2_teacher. A training iteration's gradients and
  * hessians are then sb2_distill's with weight 1, times each row's weight in a weighted dataset. Queries may have any
- * length. An id outside its query, a logit that is NaN or +inf or a log sum that is not finite returns SB2_EDATA. */
+ * length. An id outside its query, a logit that is NaN or +inf or a log sum that is not finite returns SB2_EDATA. Ranks
+ * set the teacher of their own queries, with the same temperature; training returns SB2_ECONFIG on every rank while one of
+ * them has none. */
 int sb2_set_teacher(sb2_backend* b, const int32_t* ids, const float* logits, const float* log_sum, uint64_t num_lists,
                     uint32_t top, double temperature);
 

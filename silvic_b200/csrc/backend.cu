@@ -274,8 +274,9 @@ struct sb2_backend {
         if (!loaded) return fail(SB2_EDEVICE, "b200 backend used before load");
         return SB2_OK;
     }
+    bool needs_teacher() const { return objective.kind == SB2_DISTILL && teacher.top == 0; }
     int check_teacher() {
-        if (objective.kind == SB2_DISTILL && teacher.top == 0)
+        if (needs_teacher())
             return fail(SB2_ECONFIG, "the distillation objective has no teacher (sb2_set_teacher)");
         return SB2_OK;
     }
@@ -1732,7 +1733,7 @@ int setup_training(sb2_backend* b, const sb2_params* p, double init_score, Train
          p->lambdarank_truncation_level != b->objective.lambdarank_truncation_level ||
          label_gains(p->label_gain, p->num_label_gain) != b->rank_gain))
         return b->fail(SB2_ECONFIG, "lambdarank parameters differ from the loaded objective's");
-    SB2_TRY(b->check_teacher());
+    if (!b->comm) SB2_TRY(b->check_teacher());  // ranks agree on it below, so that none waits for one that has none
     if (!p->use_quantized_grad) return b->fail(SB2_EUNSUPPORTED, "the device trainer is quantized only");
     if (p->bagging_fraction < 1.0 && p->bagging_freq > 0)
         return b->fail(SB2_EUNSUPPORTED, "bagging in the device trainer");
@@ -1782,13 +1783,18 @@ int setup_training(sb2_backend* b, const sb2_params* p, double init_score, Train
     SB2_CUDA(b, cudaMemsetAsync(b->iter.ptr, 0, sizeof(IterState), b->stream));
     SB2_CUDA(b, cudaMemsetAsync(b->counter.ptr, 0, sizeof(unsigned int), b->stream));
     if (b->comm) {
+        // The ranks' rows, and how many ranks have no teacher (each sets its own).
+        int64_t sums[2] = {global_rows, b->needs_teacher() ? 1 : 0};
         DeviceBuffer cnt;
-        SB2_CUDA(b, cnt.alloc(sizeof(int64_t)));
-        SB2_CUDA(b, cudaMemcpyAsync(cnt.ptr, &global_rows, sizeof(int64_t), cudaMemcpyHostToDevice, b->stream));
-        SB2_TRY(nccl_status(b, ncclAllReduce(cnt.ptr, cnt.ptr, 1, ncclInt64, ncclSum, b->comm, b->stream),
+        SB2_CUDA(b, cnt.alloc(sizeof(sums)));
+        SB2_CUDA(b, cudaMemcpyAsync(cnt.ptr, sums, sizeof(sums), cudaMemcpyHostToDevice, b->stream));
+        SB2_TRY(nccl_status(b, ncclAllReduce(cnt.ptr, cnt.ptr, 2, ncclInt64, ncclSum, b->comm, b->stream),
                             "ncclAllReduce(rows)"));
-        SB2_CUDA(b, cudaMemcpyAsync(&global_rows, cnt.ptr, sizeof(int64_t), cudaMemcpyDeviceToHost, b->stream));
+        SB2_CUDA(b, cudaMemcpyAsync(sums, cnt.ptr, sizeof(sums), cudaMemcpyDeviceToHost, b->stream));
         SB2_TRY(b->sync());
+        SB2_TRY(b->check_teacher());
+        if (sums[1] != 0) return b->fail(SB2_ECONFIG, "another rank has no teacher (sb2_set_teacher)");
+        global_rows = sums[0];
     }
     // Scores start at the initial score (Backend::init_scores).
     SB2_TRY(sb2_init_scores(b, 0, init_score));
