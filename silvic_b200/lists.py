@@ -15,6 +15,7 @@ import numpy as np
 from . import _abi
 
 MAX_TOP = 128  # most alternatives of a list, and most entries of a teacher's top
+MAX_LISTS = 2 ** 32 - 1  # of one call
 
 
 @dataclass
@@ -104,6 +105,8 @@ def lists_arg(scores, boundaries) -> _abi.Lists:
         if scores.dim() != 2:
             raise ValueError("scores: a 2-D tensor, or a 1-D one with boundaries")
         rows, cols = scores.shape
+        if rows > MAX_LISTS:
+            raise ValueError(f"{rows} lists; {MAX_LISTS} at most in one call")
         return _abi.Lists(scores.data_ptr(), code, rows, cols, _row_stride(scores, "scores"), None)
     torch = _torch
     if scores.dim() != 1 or (scores.shape[0] > 1 and scores.stride(0) != 1):
@@ -111,6 +114,8 @@ def lists_arg(scores, boundaries) -> _abi.Lists:
     if boundaries.dim() != 1 or boundaries.shape[0] < 1 or boundaries.dtype not in (torch.int32, torch.uint32) \
             or not boundaries.is_contiguous():
         raise ValueError("boundaries: a contiguous 1-D int32 or uint32 tensor of one entry more than lists")
+    if boundaries.shape[0] - 1 > MAX_LISTS:
+        raise ValueError(f"{boundaries.shape[0] - 1} lists; {MAX_LISTS} at most in one call")
     return _abi.Lists(scores.data_ptr(), code, boundaries.shape[0] - 1, scores.shape[0], 0, boundaries.data_ptr())
 
 
