@@ -598,8 +598,8 @@ void launch_typed(const LogProbsArgs& a, cudaStream_t s) {
     constexpr int kVec = 16 / sizeof(T);
     const uint64_t mean = a.l.bounds != nullptr ? a.l.width / a.l.lists : a.l.width;
     if (mean <= (a.l.bounds != nullptr ? kWarpMean : kWarpEntries)) {
-        const uint32_t lists = kWarpThreads / 32;
-        log_probs_warps_kernel<T><<<(a.l.lists + lists - 1) / lists, kWarpThreads, 0, s>>>(a);
+        const uint32_t lists = kWarpThreads / 32, grid = a.l.lists / lists + (a.l.lists % lists != 0);
+        log_probs_warps_kernel<T><<<grid, kWarpThreads, 0, s>>>(a);
         return;
     }
     const uint32_t shares = list_shares(mean, a.l.lists, a.sms);

@@ -3,6 +3,8 @@ near what f32 holds; against the definitions in 64 bits (lists_reference.py)."""
 
 from __future__ import annotations
 
+import ctypes as C
+
 import lists_reference as ref
 import numpy as np
 import pytest
@@ -254,3 +256,10 @@ def test_a_failed_load_leaves_no_dataset_behind(device):
             b.compute_gradients()
             for x, y in zip(want, b.read_gradients()):
                 assert np.array_equal(x, y)
+
+
+def test_the_most_lists_of_a_call(backend):  # noqa: F811
+    """2^32 - 1 lists without entries and without outputs: nothing is written, and nothing is refused."""
+    lists = _abi.Lists(None, _abi.F32, 2 ** 32 - 1, 0, 0, None)
+    backend._check(backend._lib.sb2_log_probs(backend._h, C.byref(lists), 1.0, None, 0, 0, None, None, None, None, None, None))
+    torch.cuda.synchronize()
