@@ -414,7 +414,7 @@ int sb2_set_dominant_share(sb2_backend* b, double share);
  * operators that make a teacher of the first and a student of the second. A list is a row of a dense matrix (one
  * position's logits over a vocabulary) or a run of a flat array between two boundaries (a query's documents).
  *
- * Every pointer named _dev is memory of the handle's device (else SB2_EDATA). The calls enqueue one kernel on `stream`
+ * Every pointer named _dev is memory of the handle's device, aligned to its entries (else SB2_EDATA). The calls enqueue one kernel on `stream`
  * (a cudaStream_t of that device; NULL: its default stream), allocate nothing, wait for nothing, and may be captured
  * into a CUDA graph; the caller orders them after the writes of their inputs. Calls on different streams do not
  * disturb one another. The current device stays as it was.

@@ -2266,9 +2266,12 @@ struct DeviceScope {
     }
 };
 
-// Memory that a kernel of the handle's device may use: its device's own, or managed.
-int check_memory(sb2_backend* b, const void* p, const char* what) {
+uint64_t type_bytes(int32_t type) { return type == SB2_F32 ? 4 : 2; }
+
+// Memory that a kernel of the handle's device may use: its device's own, or managed, aligned to its entries (`bytes` each).
+int check_memory(sb2_backend* b, const void* p, const char* what, uint64_t bytes = 4) {
     if (!p) return b->fail(SB2_EDATA, std::string(what) + " is null");
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return b->fail(SB2_EDATA, std::string(what) + " is not aligned to its type");
     cudaPointerAttributes attr{};
     if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
         cudaGetLastError();
@@ -2283,8 +2286,6 @@ int check_memory(sb2_backend* b, const void* p, const char* what) {
 }
 
 int check_optional(sb2_backend* b, const void* p, const char* what) { return p ? check_memory(b, p, what) : SB2_OK; }
-
-uint64_t type_bytes(int32_t type) { return type == SB2_F32 ? 4 : 2; }
 
 int check_type(sb2_backend* b, int32_t type, const void* p, const char* what) {
     if (type != SB2_F32 && type != SB2_BF16 && type != SB2_F16)
@@ -2316,7 +2317,7 @@ int list_args(sb2_backend* b, const sb2_lists* lists, ListsArgs& a) {
             return b->fail(SB2_EUNSUPPORTED, std::to_string(lists->width) + " entries behind boundaries; the limit is 2^31 - 1");
         SB2_TRY(check_memory(b, lists->boundaries_dev, "the boundaries"));
     }
-    if (lists->num_lists > 0 && lists->width > 0) SB2_TRY(check_memory(b, lists->scores_dev, "the scores"));
+    if (lists->num_lists > 0 && lists->width > 0) SB2_TRY(check_memory(b, lists->scores_dev, "the scores", type_bytes(lists->type)));
     a.scores = lists->scores_dev;
     a.type = lists->type;
     a.lists = lists->num_lists;
@@ -2397,7 +2398,7 @@ int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* tea
     if (a.l.lists == 0) return SB2_OK;
     SB2_TRY(check_type(b, teacher->type, teacher->logits_dev, "the teacher's logits"));
     SB2_TRY(check_memory(b, teacher->ids_dev, "the teacher's ids"));
-    SB2_TRY(check_memory(b, teacher->logits_dev, "the teacher's logits"));
+    SB2_TRY(check_memory(b, teacher->logits_dev, "the teacher's logits", type_bytes(teacher->type)));
     SB2_TRY(check_optional(b, teacher->log_sum_dev, "the teacher's log sums"));
     SB2_TRY(check_optional(b, weight_dev, "the weights"));
     SB2_TRY(check_optional(b, loss_dev, "the loss"));
@@ -2409,7 +2410,7 @@ int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* tea
     for (const void* out : {static_cast<const void*>(grad_dev), static_cast<const void*>(hess_dev)}) {
         if (!out || a.l.width == 0) continue;
         SB2_TRY(check_type(b, a.l.type, out, "the gradients"));
-        SB2_TRY(check_memory(b, out, "the gradients"));
+        SB2_TRY(check_memory(b, out, "the gradients", type_bytes(a.l.type)));
         if (overlap(a.l.scores, extent(a.l, a.l.stride), out, extent(a.l, grad_stride)))
             return b->fail(SB2_EDATA, "the gradients overlap the scores");
     }

@@ -263,3 +263,34 @@ def test_the_most_lists_of_a_call(backend):  # noqa: F811
     lists = _abi.Lists(None, _abi.F32, 2 ** 32 - 1, 0, 0, None)
     backend._check(backend._lib.sb2_log_probs(backend._h, C.byref(lists), 1.0, None, 0, 0, None, None, None, None, None, None))
     torch.cuda.synchronize()
+
+
+def test_misaligned_pointers_are_refused(backend):  # noqa: F811
+    """Every pointer of 4-byte entries, 2 bytes off; the calls are refused before a launch."""
+    x = torch.zeros(4096, device="cuda")
+    ok, off = x.data_ptr(), x.data_ptr() + 4096 + 2
+    lists = _abi.Lists(ok, _abi.F32, 2, 8, 8, None)
+    runs = _abi.Lists(ok, _abi.F32, 2, 8, 0, off)
+    lib, h = backend._lib, backend._h
+
+    def log_probs(a=lists, **at):
+        p = dict(given=ok + 1024, given_out=ok + 2048, entropy=ok + 3072, log_sum=ok + 4096, ids=ok + 5120, out=ok + 6144)
+        p.update(at)
+        return lib.sb2_log_probs(h, C.byref(a), 1.0, p["given"], 1, 2, p["given_out"], p["entropy"], p["log_sum"], p["ids"], p["out"],
+                                 None)
+
+    def distill(a=lists, **at):
+        p = dict(ids=ok + 1024, log_sum=ok + 2048, weight=ok + 3072, loss=ok + 4096)
+        p.update(at)
+        t = _abi.Teacher(p["ids"], ok + 512, _abi.F32, 2, 2, p["log_sum"])
+        return lib.sb2_distill(h, C.byref(a), C.byref(t), 1.0, p["weight"], p["loss"], None, None, 0, None)
+
+    for call, names in ((log_probs, ("given", "given_out", "entropy", "log_sum", "ids", "out")),
+                        (distill, ("ids", "log_sum", "weight", "loss"))):
+        assert call(runs) == _abi.EDATA
+        for name in names:
+            assert call(**{name: off}) == _abi.EDATA, name
+            with pytest.raises(SilvicError, match="aligned"):
+                backend._check(call(**{name: off}))
+        assert call() == _abi.OK
+    torch.cuda.synchronize()
