@@ -201,7 +201,10 @@ def check_device(device: int, tensors):
 
 def host_teacher(teacher: TeacherTop):
     """(ids, logits, log_sum or None) of a training teacher as C-contiguous numpy arrays."""
-    ids = np.ascontiguousarray(teacher.ids, dtype=np.int32)
+    ids = np.asarray(teacher.ids)
+    if ids.size and (ids.dtype.kind not in "iu" or ids.min() < -2 ** 31 or ids.max() >= 2 ** 31):
+        raise ValueError(f"the teacher's ids: whole numbers of 32 bits, not {ids.dtype} from {ids.min()} to {ids.max()}")
+    ids = np.ascontiguousarray(ids, dtype=np.int32)
     logits = np.ascontiguousarray(teacher.logits, dtype=np.float32)
     if ids.ndim != 2 or ids.shape != logits.shape:
         raise ValueError(f"a teacher of ids {ids.shape} and logits {logits.shape}")
