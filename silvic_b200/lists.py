@@ -89,6 +89,8 @@ def _row_stride(tensor, what: str) -> int:
     """Entries from one row of a 2-D tensor to the next; its rows are contiguous and lie apart."""
     rows, cols = tensor.shape
     step, one = tensor.stride()
+    if rows == 0 or cols == 0:  # whatever its strides
+        return cols
     if cols > 1 and one != 1:
         raise ValueError(f"{what}: rows of contiguous entries")
     if rows <= 1:

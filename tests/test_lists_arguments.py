@@ -29,3 +29,12 @@ def test_a_training_teacher_s_ids_are_not_cut():
         with pytest.raises(ValueError, match="ids"):
             lists.host_teacher(TeacherTop(np.array(bad), logits))
     assert lists.host_teacher(TeacherTop(np.zeros((0, 3)), np.zeros((0, 3))))[0].shape == (0, 3)
+
+
+def test_tensors_without_entries_are_taken_whatever_their_strides():
+    for shape in ((0, 4), (4, 0), (0, 0)):
+        for strides in ((1, 1), (0, 7), (3, 2)):
+            arg = lists.lists_arg(torch.empty_strided(shape, strides), None)
+            assert (arg.num_lists, arg.width, arg.stride) == (shape[0], shape[1], shape[1])
+    t, _ = lists.teacher_arg(TeacherTop(torch.empty_strided((0, 4), (1, 1), dtype=torch.int32), torch.empty(0, 4)), 0)
+    assert (t.top, t.stride) == (4, 4)
