@@ -414,10 +414,10 @@ int sb2_set_dominant_share(sb2_backend* b, double share);
  * operators that make a teacher of the first and a student of the second. A list is a row of a dense matrix (one
  * position's logits over a vocabulary) or a run of a flat array between two boundaries (a query's documents).
  *
- * Every pointer named _dev is memory of the handle's device, aligned to its entries (else SB2_EDATA). The calls enqueue one kernel on `stream`
- * (a cudaStream_t of that device; NULL: its default stream), allocate nothing, wait for nothing, and may be captured
- * into a CUDA graph; the caller orders them after the writes of their inputs. Calls on different streams do not
- * disturb one another. The current device stays as it was.
+ * Every pointer named _dev is memory of the handle's device, aligned to its entries (else SB2_EDATA). The calls enqueue
+ * one kernel on `stream` (a cudaStream_t of that device; NULL: its default stream), allocate nothing, wait for nothing,
+ * and may be captured into a CUDA graph; the caller orders them after the writes of their inputs. Calls on different
+ * streams do not disturb one another. The current device stays as it was.
  *
  * Values: -inf is a masked entry (probability 0); a list that holds a NaN or +inf has NaN results; -0 equals 0. A list
  * of no entries, or of masked ones only, is empty: log sum -inf, entropy 0, no alternatives, loss and gradients 0.
@@ -464,8 +464,9 @@ int sb2_log_probs(sb2_backend* b, const sb2_lists* lists, double temperature, co
  *   grad_dev              d loss / d z_j = weight / T * (Q p_j - q_j) in the top, weight / T * p_j (Q - r / P) elsewhere
  *   hess_dev              weight / T^2 * Q p_j (1 - p_j), the diagonal of the softmax's own second derivative
  * weight_dev [num_lists] may be NULL (1 each), so may any of the three outputs. Gradient and hessian have the scores'
- * type; with boundaries their layout too, dense rows start grad_stride entries apart (0: as the scores'), and entries
- * between the lists stay as they are. They must not overlap the scores or each other (SB2_EDATA). A list whose
+ * type; with boundaries their layout too, dense rows start grad_stride entries apart (0: as the scores'). Entries between
+ * dense rows, before the first list and behind the last stay as they are; with boundaries and a grad_stride of 1 those in
+ * no list are set to 0. They must not overlap the scores or each other (SB2_EDATA). A list whose
  * teacher has no entry in it has loss and gradients 0; a teacher's entry that the student masks has loss +inf. */
 int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* teacher, double temperature,
                 const float* weight_dev, float* loss_dev, void* grad_dev, void* hess_dev, uint64_t grad_stride,

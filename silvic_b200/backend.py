@@ -288,8 +288,9 @@ class B200Backend:
         """The distillation loss of every list against a teacher's top logits, its gradient and the softmax's own
         hessian diagonal with respect to `scores` (`sb2_distill`, which has the formulas). `scores` and `boundaries`
         as in `log_probs`; `weight` (f32 [lists]) multiplies a list's loss and derivatives (a loss's upstream
-        gradient, say). Gradient and hessian have the scores' type and shape, in memory of their own. Runs on torch's
-        current stream of the handle's device, without waiting; may be captured into a graph."""
+        gradient, say). Gradient and hessian have the scores' type and shape, in memory of their own, and are 0 for
+        entries of no list. Runs on torch's current stream of the handle's device, without waiting; may be captured
+        into a graph."""
         arg = _lists.lists_arg(scores, boundaries)
         n = arg.num_lists
         t, keep = _lists.teacher_arg(teacher, n)
@@ -299,7 +300,7 @@ class B200Backend:
         loss = scores.new_empty(n, dtype=_lists.torch_float32())
         # Gradients of padded rows are padded alike, so that both sides' rows start on the same boundaries; rows cut
         # from far wider ones (a stride of more than the width and 64) lie one behind the other.
-        stride = 0 if boundaries is not None else arg.stride if arg.stride <= arg.width + 64 else arg.width
+        stride = 1 if boundaries is not None else arg.stride if arg.stride <= arg.width + 64 else arg.width
         grad = _lists.like(scores, n, arg.width, stride) if gradient else None
         hess = _lists.like(scores, n, arg.width, stride) if hessian else None
         self._check(self._lib.sb2_distill(self._h, arg, t, teacher.temperature, None if weight is None else weight.data_ptr(),

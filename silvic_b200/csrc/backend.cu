@@ -2425,6 +2425,7 @@ int sb2_distill(sb2_backend* b, const sb2_lists* student, const sb2_teacher* tea
     a.inv_t = static_cast<float>(1.0 / temperature);
     a.sms = static_cast<uint32_t>(b->sms);
     a.grad_stride = grad_stride;
+    a.clear = a.l.bounds != nullptr && grad_stride == 1 && (grad_dev || hess_dev);
     a.weight = weight_dev;
     a.loss = loss_dev;
     a.grad = grad_dev;

@@ -256,6 +256,22 @@ __device__ __forceinline__ uint32_t marks_of(const Shared<kThreads>& s, const ui
     return m;
 }
 
+// Derivatives 0 for the entries before the first list and behind the last, by the first kClearing CTAs: they are through
+// before the others, so that few calls wait for the loads of the two boundaries.
+constexpr uint32_t kClearing = 64;
+template <class T>
+__device__ __forceinline__ void clear_ends(const DistillArgs& a) {
+    if (!a.clear || blockIdx.x >= kClearing) return;
+    const uint64_t begin = a.l.bounds[0], end = a.l.bounds[a.l.lists];
+    const uint64_t low = begin < a.l.width ? begin : a.l.width, high = end < low ? low : end < a.l.width ? end : a.l.width;
+    const uint64_t count = low + (a.l.width - high), step = min(gridDim.x, kClearing) * static_cast<uint64_t>(blockDim.x);
+    for (uint64_t j = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; j < count; j += step) {
+        const uint64_t at = j < low ? j : high + (j - low);
+        if (a.grad != nullptr) static_cast<T*>(a.grad)[at] = from_float<T>(0.0f);
+        if (a.hess != nullptr) static_cast<T*>(a.hess)[at] = from_float<T>(0.0f);
+    }
+}
+
 // What is on its way for a CTA's next list while this one's gradients are written.
 struct Ahead {
     bool flying = false;  // the scores, into the threads' slots, and the thread's entry of the teacher
@@ -886,6 +902,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(
         distill_list<T, kVec, kThreads, kCluster>(s, data, slots, bits, a, i, i + step, ahead, blockIdx.x & (shares - 1), shares, most);
         __syncthreads();  // what the list left in shared memory is read
     }
+    if (kVec == 1) clear_ends<T>(a);
     publish<kThreads>(a, most);
 }
 
@@ -1108,6 +1125,7 @@ __global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4) distill_warp
             distill_list<T, 1, kWarpThreads, false>(shared, nullptr, 0, bits, a, k, a.l.lists, ahead, 0, 1, most);
             __syncthreads();
         }
+    clear_ends<T>(a);
     publish<kWarpThreads>(a, most);
 }
 

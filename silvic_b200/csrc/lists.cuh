@@ -53,6 +53,7 @@ struct DistillArgs {
     float* loss;               // [lists] or nullptr
     void* grad;                // scores' type and layout, or nullptr
     void* hess;                // scores' type and layout, or nullptr
+    bool clear;                // with bounds: entries of no list have derivatives 0
     // a training iteration's gradients only (f32):
     const float* row_weight;   // per entry, or nullptr
     const int32_t* stopped;    // nothing is done when set

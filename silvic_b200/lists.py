@@ -149,8 +149,8 @@ class Outputs:
 
 def like(scores, rows: int, width: int, stride: int):
     """Memory for derivatives of `scores`: rows `stride` entries apart, or (1-D scores) a flat copy of it."""
-    if scores.dim() == 1:
-        return scores.new_empty(scores.shape[0])
+    if scores.dim() == 1:  # (without lists nothing is launched)
+        return scores.new_empty(scores.shape[0]) if rows > 0 else scores.new_zeros(scores.shape[0])
     if stride == width:
         return scores.new_empty((rows, width))
     return scores.new_empty((rows, stride)).as_strided((rows, width), (stride, 1))

@@ -294,3 +294,27 @@ def test_misaligned_pointers_are_refused(backend):  # noqa: F811
                 backend._check(call(**{name: off}))
         assert call() == _abi.OK
     torch.cuda.synchronize()
+
+
+# ---- entries of no list --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("bounds,total", [([3, 40, 60], 200), ([0, 700, 700, 1200], 1201), ([5], 9), ([2000, 9000], 300_000),
+                                          ([0, 5000, 9001], 9001), ([7, 7, 7], 11), ([0, 90_000], 90_000),
+                                          ([1, 60_000, 130_001], 130_005)])
+def test_entries_of_no_list_have_gradient_0(backend, bounds, total, type_):  # noqa: F811
+    """The tensors' memory held other values before: what is before the first list and behind the last is 0."""
+    rng = np.random.RandomState(total)
+    scores = torch.from_numpy(rng.randn(total)).to(TYPES[type_]).cuda()
+    sizes = np.diff(bounds)
+    teacher = random_teacher(rng, sizes, 4)
+    for _ in range(3):
+        junk = [torch.full((total,), float("nan"), dtype=TYPES[type_], device="cuda") for _ in range(4)]
+        del junk
+        got = backend.distill(scores, teacher, boundaries=torch.tensor(bounds, dtype=torch.int32, device="cuda"), hessian=True)
+        for v in (got.gradient, got.hessian):
+            assert v.shape == (total,)
+            assert (v[: bounds[0]] == 0).all() and (v[bounds[-1]:] == 0).all()
+        if len(sizes):
+            check_distill(scores, teacher, got, None, bounds, type_)
