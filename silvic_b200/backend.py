@@ -275,13 +275,17 @@ class B200Backend:
         if not 0 <= top <= _lists.MAX_TOP:
             raise ValueError(f"{top} alternatives; 0 to {_lists.MAX_TOP} are given")
         _lists.check_device(self._device, (scores, boundaries, given))
-        # The outputs in one allocation, whose parts start at multiples of 4 bytes.
-        made = _lists.Outputs(scores, n, (num_given, 1, 1, top, top))
-        at = made.pointers
+        entropy, log_sum = _lists.output(scores, n), _lists.output(scores, n)
+        given_out = _lists.output(scores, n, num_given) if num_given else None
+        top_ids = _lists.output(scores, n, top, ids=True) if top else None
+        top_out = _lists.output(scores, n, top) if top else None
         self._check(self._lib.sb2_log_probs(self._h, arg, temperature, given.data_ptr() if num_given else None, num_given,
-                                            top, at[0], at[1], at[2], at[3], at[4], _lists.stream(self._device)))
-        return LogProbs(made.part(0) if given is not None else None, made.flat(1), made.flat(2),
-                        made.ids(3) if top else None, made.part(4) if top else None)
+                                            top, given_out.data_ptr() if num_given else None, entropy.data_ptr(),
+                                            log_sum.data_ptr(), top_ids.data_ptr() if top else None,
+                                            top_out.data_ptr() if top else None, _lists.stream(self._device)))
+        if given is not None and num_given == 0:
+            given_out = scores.new_empty((n, 0), dtype=_lists.torch_float32())
+        return LogProbs(given_out, entropy, log_sum, top_ids, top_out)
 
     def distill(self, scores, teacher: TeacherTop, *, boundaries=None, weight=None, gradient: bool = True,
                 hessian: bool = False) -> Distilled:

@@ -121,30 +121,11 @@ def lists_arg(scores, boundaries) -> _abi.Lists:
     return _abi.Lists(scores.data_ptr(), code, boundaries.shape[0] - 1, scores.shape[0], 0, boundaries.data_ptr())
 
 
-class Outputs:
-    """f32 and int32 outputs of `columns` values a list each, in one allocation beside the scores: a call's host time
-    is a few microseconds, and an allocation is the largest part of it."""
-
-    def __init__(self, scores, rows: int, columns):
-        self._rows, self._columns, self._starts = rows, columns, []
-        total = 0
-        for c in columns:
-            self._starts.append(total)
-            total += rows * c
-        self._buffer = scores.new_empty(total, dtype=_torch.float32)
-        base = self._buffer.data_ptr()
-        self.pointers = [base + 4 * s if rows * c else None for s, c in zip(self._starts, columns)]
-
-    def part(self, i: int):
-        c = self._columns[i]
-        return self._buffer.as_strided((self._rows, c), (c, 1), self._starts[i])
-
-    def flat(self, i: int):
-        return self._buffer.as_strided((self._rows,), (1,), self._starts[i])
-
-    def ids(self, i: int):
-        c = self._columns[i]
-        return self._buffer.view(_torch.int32).as_strided((self._rows, c), (c, 1), self._starts[i])
+def output(scores, rows: int, columns: int = 0, ids: bool = False):
+    """Memory for an output beside the scores, f32 or int32 [rows, columns], [rows] without columns. One of its own each,
+    so that what is done to one output in place, or how long it is kept, is no matter of the others'."""
+    return _torch.empty_strided((rows, columns) if columns else (rows,), (columns, 1) if columns else (1,),
+                                dtype=_torch.int32 if ids else _torch.float32, device=scores.device)
 
 
 def like(scores, rows: int, width: int, stride: int):

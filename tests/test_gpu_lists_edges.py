@@ -318,3 +318,23 @@ def test_entries_of_no_list_have_gradient_0(backend, bounds, total, type_):  # n
             assert (v[: bounds[0]] == 0).all() and (v[bounds[-1]:] == 0).all()
         if len(sizes):
             check_distill(scores, teacher, got, None, bounds, type_)
+
+
+# ---- outputs -------------------------------------------------------------------------------------------------------
+
+
+def test_outputs_are_tensors_of_their_own(backend):  # noqa: F811
+    """What is done to one in place leaves the others, and what autograd saved of them, alone."""
+    x = torch.randn(5, 900, device="cuda")
+    got = backend.log_probs(x, given=torch.zeros(5, 2, dtype=torch.int32, device="cuda"), top=3)
+    parts = [got.given, got.entropy, got.log_sum, got.top_ids, got.top]
+    assert len({v.untyped_storage().data_ptr() for v in parts}) == 5
+    assert [v.untyped_storage().nbytes() for v in parts] == [40, 20, 20, 60, 60] and all(v.is_contiguous() for v in parts)
+    w = torch.ones(5, 2, device="cuda", requires_grad=True)
+    loss = (w * got.given).sum()
+    got.entropy.mul_(2.0)
+    got.top.add_(1.0)
+    loss.backward()
+    assert torch.equal(w.grad, got.given)
+    none = backend.log_probs(x, given=torch.zeros(5, 0, dtype=torch.int32, device="cuda"))
+    assert none.given.shape == (5, 0) and none.top is None and none.top_ids is None
