@@ -233,6 +233,17 @@ __device__ __forceinline__ bool expand(Shared<kThreads>& s, const T* z, float bo
     return s.keys <= kCandidates;
 }
 
+// A given entry's score, -inf for an index outside the list.
+template <class T>
+__device__ __forceinline__ float given_score(const T* z, uint32_t n, int32_t id) {
+    return id >= 0 && static_cast<uint32_t>(id) < n ? to_float(z[id]) : -CUDART_INF_F;
+}
+// ... and its log probability: a masked entry's is -inf, but NaN beside a NaN or +inf as all of that list's.
+__device__ __forceinline__ float given_log_prob(float z, uint32_t n, int32_t id, float m, float inv_t, float log_s) {
+    if (z == -CUDART_INF_F) return log_s == log_s || id < 0 || static_cast<uint32_t>(id) >= n ? z : log_s;
+    return (z - m) * inv_t - log_s;
+}
+
 // One list by `shares` CTAs, this one the `share`-th: a cluster, or a CTA alone (shares 1).
 template <class T, int kVec, int kThreads, bool kCluster>
 __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogProbsArgs& a, uint32_t i, uint32_t share,
@@ -246,11 +257,9 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(w.vectors) * (share + 1) / shares);
     const float c = __fmul_rn(kLog2E, a.inv_t);
     // The given entries' scores, on their way while the list is read.
-    float given = -CUDART_INF_F;
-    if (share == 0 && t < a.num_given) {
-        const int32_t id = a.given[static_cast<uint64_t>(i) * a.num_given + t];
-        if (id >= 0 && static_cast<uint32_t>(id) < n) given = to_float(w.z[id]);
-    }
+    int32_t id = -1;
+    if (share == 0 && t < a.num_given) id = a.given[static_cast<uint64_t>(i) * a.num_given + t];
+    float given = given_score(w.z, n, id);
     // The first batch, and the scalars outside the vectors (share 0): their maximum.
     Pack<T, kVec> p[kBatch];
 #pragma unroll
@@ -412,10 +421,10 @@ __device__ __forceinline__ void log_probs_list(Shared<kThreads>& s, const LogPro
     for (uint32_t g = t; g < a.num_given; g += kThreads) {
         const uint64_t at = static_cast<uint64_t>(i) * a.num_given + g;
         if (g >= kThreads) {
-            const int32_t id = a.given[at];
-            given = id >= 0 && static_cast<uint32_t>(id) < n ? to_float(w.z[id]) : -CUDART_INF_F;
+            id = a.given[at];
+            given = given_score(w.z, n, id);
         }
-        a.given_out[at] = given == -CUDART_INF_F ? given : (given - m) * a.inv_t - log_s;
+        a.given_out[at] = given_log_prob(given, n, id, m, a.inv_t, log_s);
     }
     for (uint32_t k = t; k < a.top; k += kThreads) {
         const uint64_t at = static_cast<uint64_t>(i) * a.top + k;
@@ -465,8 +474,7 @@ __device__ __forceinline__ void log_probs_warp(const LogProbsArgs& a, uint32_t i
     for (uint32_t g = lane; g < a.num_given; g += 32) {
         const uint64_t at = static_cast<uint64_t>(i) * a.num_given + g;
         const int32_t id = a.given[at];
-        const float given = id >= 0 && static_cast<uint32_t>(id) < n ? to_float(z[id]) : -CUDART_INF_F;
-        a.given_out[at] = given == -CUDART_INF_F ? given : (given - m) * a.inv_t - log_s;
+        a.given_out[at] = given_log_prob(given_score(z, n, id), n, id, m, a.inv_t, log_s);
     }
     // The alternatives, one a round: each lane keeps its entries in order and offers the first that is left.
     if (a.top == 0) return;

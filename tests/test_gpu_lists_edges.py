@@ -338,3 +338,26 @@ def test_outputs_are_tensors_of_their_own(backend):  # noqa: F811
     assert torch.equal(w.grad, got.given)
     none = backend.log_probs(x, given=torch.zeros(5, 0, dtype=torch.int32, device="cuda"))
     assert none.given.shape == (5, 0) and none.top is None and none.top_ids is None
+
+
+# ---- given entries -------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("given", [3, 700])
+@pytest.mark.parametrize("lists,width", [(6, 300), (6, 1000), (300, 5001), (6, 70001)])
+def test_given_entries_of_every_kind(backend, lists, width, given):  # noqa: F811
+    """More given entries than a CTA has threads; masked ones and indices outside the list, in lists with a NaN or +inf
+    (all of their log probabilities are NaN), in empty ones and in others."""
+    rng = np.random.RandomState(width + given)
+    z = rng.randn(lists, width) * 3
+    z[:, : width // 3] = -np.inf
+    z[0, -1] = np.nan
+    z[1, width // 2] = np.inf
+    z[2] = -np.inf
+    scores = torch.from_numpy(z).float().cuda()
+    ids = rng.randint(0, width, (lists, given)).astype(np.int32)
+    ids[:, 0], ids[:, 1], ids[:, 2] = 0, -1, width  # masked; outside
+    got = backend.log_probs(scores, given=torch.from_numpy(ids).cuda(), top=4)
+    check_log_probs(scores[:6], rows_of(scores[:6]), ids, 4, 1.0,
+                    type(got)(*[v[:6] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
+    assert torch.isnan(got.given[:2, 0]).all() and (got.given[:, 1:3] == -np.inf).all() and (got.given[2] == -np.inf).all()
