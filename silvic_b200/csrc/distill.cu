@@ -158,12 +158,18 @@ __device__ __forceinline__ uint4 packed(const float (&v)[kVec]) {
     }
 }
 
-// One entry of the teacher's top: its index (-1: padding), t / T and the student's score there.
+// ln q of a teacher's entry, up to the top's own sum without a log sum: then from the largest logit, so that a constant
+// on all of a list's logits, however large, changes nothing.
+__device__ __forceinline__ float log_q_of(float logit, float inv_t, bool rest, float log_sum, float most) {
+    return rest ? __fmaf_rn(logit, inv_t, -log_sum) : (logit - most) * inv_t;
+}
+
+// One entry of the teacher's top: its index (-1: padding) and logit.
 __device__ __forceinline__ void teacher_entry(const DistillArgs& a, uint32_t i, uint32_t k, uint32_t n, int32_t& id, float& y) {
     const uint64_t at = static_cast<uint64_t>(i) * a.t.stride + k;
     id = a.t.ids[at];
     if (id < 0 || static_cast<uint32_t>(id) >= n) id = -1;
-    y = id >= 0 ? load_typed(a.t.logits, a.t.type, at) * a.inv_t : -CUDART_INF_F;
+    y = id >= 0 ? load_typed(a.t.logits, a.t.type, at) : -CUDART_INF_F;
 }
 
 // The loss of a list from its parts: sum q (log q - (z - m) / T), sum q, S, log (S P), and the rest.
@@ -506,15 +512,15 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     bool leads = mine, alone = true;  // the first of the teacher's entries that names this index, and the only one
     if (s.again != 0 && t < a.t.top) lead(s, id, t, a.t.top, leads, alone);
     // The teacher's terms, not yet divided by their sum where the top is all of it.
-    const float base = rest ? log_sum : y_max;
-    float q = id >= 0 ? expf(y - base) : 0.0f;
+    const float log_q = log_q_of(y, a.inv_t, rest, log_sum, y_max);
+    float q = id >= 0 ? expf(log_q) : 0.0f;
     sum = warp_sum(sum);
     if (lane == 0) s.warp[2][warp] = sum;
     if (warp * 32 < a.t.top) {
         s.q[t] = q;
         const float top_part = warp_sum(rest && leads ? term(zt) : 0.0f);
         const float held_part = warp_sum(q);
-        const float cross_part = warp_sum(q != 0.0f ? q * (y - base - (zt - m) * a.inv_t) : 0.0f);
+        const float cross_part = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
         if (lane == 0) {
             s.warp[3][warp] = top_part;
             s.warp[4][warp] = held_part;
@@ -810,7 +816,6 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
     }
     // The teacher's terms about the first reference, the sums about the largest.
     m = fmaxf(m, -FLT_MAX);
-    const float base = rest ? log_sum : y_max;
     Stats mine_sum = r.stats();
     const float warp_m = warp_max(mine_sum.m);
     rebase(mine_sum, warp_m, c);
@@ -818,10 +823,10 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
     if (warp * 32 < a.t.top) {
         bool leads = mine, alone = true;
         if (rest && s.again != 0 && t < a.t.top) lead(s, id, t, a.t.top, leads, alone);
-        const float q = id >= 0 ? expf(y - base) : 0.0f;
+        const float log_q = log_q_of(y, a.inv_t, rest, log_sum, y_max), q = id >= 0 ? expf(log_q) : 0.0f;
         const float top_part = warp_sum(rest && leads ? pow2(exponent(zt, m, c)) : 0.0f);
         const float held_part = warp_sum(q);
-        const float cross_part = warp_sum(q != 0.0f ? q * (y - base - (zt - m) * a.inv_t) : 0.0f);
+        const float cross_part = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
         if (lane == 0) {
             s.warp[3][warp] = top_part;
             s.warp[4][warp] = held_part;
@@ -986,7 +991,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
             s.id[k] = id[u];
         }
         if (id[u] >= 0) {
-            y[u] = logits[u] * a.inv_t;
+            y[u] = logits[u];
             zt[u] = to_float(z[id[u]]);
             const uint32_t mark = 1u << (id[u] & 31);
             again |= (atomicOr(&s.bits[id[u] / 32], mark) & mark) != 0;
@@ -1024,7 +1029,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         leads |= first_one ? 1u << u : 0u;
         alone |= only ? 1u << u : 0u;
         if (rest && first_one) top_sum += pow2(exponent(zt[u], m, c));
-        if (!rest && id[u] >= 0) total += expf(y[u] - y_max);
+        if (!rest && id[u] >= 0) total += expf(log_q_of(y[u], a.inv_t, rest, 0.0f, y_max));
     }
     const float outside = warp_sum(sum);
     if (rest) {
@@ -1038,7 +1043,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
 #pragma unroll
     for (int u = 0; u < kTop; ++u) {
         float log_q = -CUDART_INF_F;
-        if (id[u] >= 0) log_q = rest ? y[u] - log_sum : total == 0.0f ? -CUDART_INF_F : y[u] - y_max - log_total;
+        if (id[u] >= 0 && (rest || total != 0.0f)) log_q = log_q_of(y[u], a.inv_t, rest, log_sum, y_max) - (rest ? 0.0f : log_total);
         q[u] = expf(log_q);
         held += q[u];
         if (q[u] != 0.0f) cross += q[u] * (log_q - (zt[u] - m) * a.inv_t);

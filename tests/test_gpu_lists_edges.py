@@ -361,3 +361,27 @@ def test_given_entries_of_every_kind(backend, lists, width, given):  # noqa: F81
     check_log_probs(scores[:6], rows_of(scores[:6]), ids, 4, 1.0,
                     type(got)(*[v[:6] for v in (got.given, got.entropy, got.log_sum, got.top_ids, got.top)]))
     assert torch.isnan(got.given[:2, 0]).all() and (got.given[:, 1:3] == -np.inf).all() and (got.given[2] == -np.inf).all()
+
+
+# ---- a teacher's logits far from 0 ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("sizes", [[300] * 9, [1000] * 9, [5000] * 9, [40001] * 2, [9001] * 300, [5, 700, 90, 5000]])
+def test_a_constant_on_a_teacher_s_logits_changes_nothing(backend, sizes):  # noqa: F811
+    """Without a log sum: logits that are multiples of 1/8 about 0 and about 2^20 have the same differences in f32."""
+    rng = np.random.RandomState(sizes[0])
+    uneven = len(set(sizes)) > 1
+    teacher = random_teacher(rng, sizes, 40, t=1.7)
+    logits = torch.round(teacher.logits * 8) / 8
+    bounds = np.concatenate([[0], np.cumsum(sizes)])
+    if uneven:
+        scores, boundaries = torch.from_numpy(rng.randn(bounds[-1])).float().cuda(), torch.from_numpy(bounds.astype(np.int32)).cuda()
+    else:
+        scores, boundaries = torch.from_numpy(rng.randn(len(sizes), sizes[0])).float().cuda(), None
+    for gradient in (False, True):
+        near, far = [backend.distill(scores, TeacherTop(teacher.ids, logits + c, None, 1.7), boundaries=boundaries, gradient=gradient)
+                     for c in (0.0, 2.0 ** 20)]
+        assert torch.equal(near.loss, far.loss) and (not gradient or torch.equal(near.gradient, far.gradient))
+    if not uneven:
+        near = type(near)(near.loss[:9], near.gradient[:9])
+        check_distill(scores[:9], TeacherTop(teacher.ids[:9], logits[:9], None, 1.7), near)
