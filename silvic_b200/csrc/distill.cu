@@ -9,13 +9,14 @@
 //   hess_j = w / T^2 Q p_j (1 - p_j)        (the diagonal of the softmax's own second derivative)
 // P is summed over the entries outside the top, not taken as 1 - sum p: a student that has learned its teacher keeps
 // little there. Where that is less than 2^-40, the entries outside go about their own maximum in a pass of their own: f32
-// holds the gradient's r p_j / P however small P is. The top's entries are marked in a bitmap, which the sum skips; their gradients are written once the
-// others are, over what the common formula left there. An entry named twice has its q added in the teacher's order.
+// holds the gradient's r p_j / P however small P is. The top's entries are marked in a bitmap, which the sum skips; their
+// gradients are written once the others are, over what the common formula left there. An entry named twice has its q added
+// in the teacher's order.
 //
-// Lists of at most 512 entries (1024 of a dense matrix) take a warp each, in registers. A longer list takes a CTA or a cluster of CTAs that
-// holds it in shared memory between the passes (each thread its own vectors), so that memory sees each score once. Runs
-// between boundaries are read again from the caches, entry by entry, so that a list's sums do not depend on where it
-// starts. A dense list too long for shared memory, or of scores so far from 0 that fma(z, c, -m c) loses its last bits,
+// Lists of at most 512 entries (1024 of a dense matrix) take a warp each, in registers. A longer list takes a CTA or a
+// cluster of CTAs that holds it in shared memory between the passes (each thread its own vectors), so that memory sees each
+// score once. Runs between boundaries are read again from the caches, entry by entry, so that a list's sums do not depend on
+// where it starts. A dense list too long for shared memory, or of scores so far from 0 that fma(z, c, -m c) loses its last bits,
 // is read again for each pass. The loss alone is taken in one pass that holds nothing.
 //
 // What bounds it, on one B200 (copy rate 6453 GB/s): 4096 lists of 32000 bf16 scores, top 64 with the rest, take 120 us,
@@ -394,12 +395,13 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     const bool held_here = kVec == 1 || to - from <= slots, room = bits != nullptr;
     const float log_sum = rest ? a.t.log_sum[i] : 0.0f, weight = a.weight != nullptr ? a.weight[i] : 1.0f;
     // The scores, on their way to the thread's own slots.
-    if (kVec > 1 && held_here && !ahead.flying) {
-        const T* z = w.z + w.at(from);
+    if constexpr (kVec > 1)
+        if (held_here && !ahead.flying) {
+            const T* z = w.z + w.at(from);
 #pragma unroll 4
-        for (uint32_t v = t; v < to - from; v += kThreads) data[v].copy(z + static_cast<size_t>(v) * kVec);
-        copies_begun();
-    }
+            for (uint32_t v = t; v < to - from; v += kThreads) data[v].copy(z + static_cast<size_t>(v) * kVec);
+            copies_begun();
+        }
     const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
     const float edge = edge_at < n ? to_float(w.z[edge_at]) : -CUDART_INF_F;
     // The teacher, and the marks of its entries in this share.
@@ -893,7 +895,8 @@ __global__ void __launch_bounds__(kThreads) distill_loss_kernel(const __grid_con
 }
 
 template <class T, int kVec, int kThreads, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 768 / kThreads) distill_rows_kernel(const __grid_constant__ DistillArgs a, uint32_t shares, uint32_t slots) {
+__global__ void __launch_bounds__(kThreads, 768 / kThreads)
+    distill_rows_kernel(const __grid_constant__ DistillArgs a, uint32_t shares, uint32_t slots) {
     if (a.stopped != nullptr && *a.stopped) return;
     extern __shared__ __align__(16) unsigned char held[];
     __shared__ Shared<kThreads> s;
@@ -1087,10 +1090,11 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     }
 }
 
-// `per` lists a CTA (8 at most), a warp each of at most 32 kMost entries; a longer one among them by the whole CTA. So what a list gives depends on
-// its own length alone.
+// `per` lists a CTA (8 at most), a warp each of at most 32 kMost entries; a longer one among them by the whole CTA. So what
+// a list gives depends on its own length alone.
 template <class T, int kTop, int kMost>
-__global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4) distill_warps_kernel(const __grid_constant__ DistillArgs a, uint32_t per) {
+__global__ void __launch_bounds__(kWarpThreads, kMost > 16 ? 2 : 4)
+    distill_warps_kernel(const __grid_constant__ DistillArgs a, uint32_t per) {
     constexpr uint32_t kEntries = 32 * kMost;
     if (a.stopped != nullptr && *a.stopped) return;
     __shared__ WarpShared warps[kWarpThreads / 32];
@@ -1169,7 +1173,8 @@ void launch_rows(const DistillArgs& a, uint32_t shares, uint32_t slots, cudaStre
     // memory 227 KB), each taking its next list while it writes.
     uint32_t lists = a.l.lists;
     if (kVec > 1 && shares == 1) {
-        const uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(768 / kThreads, 227 * 1024 / (smem + sizeof(Shared<kThreads>) + 1024)));
+        const size_t each = smem + sizeof(Shared<kThreads>) + 1024;
+        const uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(768 / kThreads, 227 * 1024 / each));
         lists = std::min(lists, a.sms * std::max(1u, ctas));
     }
     launch_shares(shares > 1 ? distill_rows_kernel<T, kVec, kThreads, true> : distill_rows_kernel<T, kVec, kThreads, false>, a,

@@ -95,7 +95,8 @@ struct Walk {
     uint32_t n, head, vectors;
     __device__ __forceinline__ Walk(const T* scores, uint32_t entries) : z(scores), n(entries) {
         head = 0;
-        if (kVec > 1) head = min(n, static_cast<uint32_t>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / static_cast<uint32_t>(sizeof(T)));
+        const uint32_t bytes = static_cast<uint32_t>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15);  // to the boundary
+        if (kVec > 1) head = min(n, bytes / static_cast<uint32_t>(sizeof(T)));
         vectors = (n - head) / kVec;
     }
     // The first entry of vector v, and where the scalars behind the vectors start.
@@ -201,17 +202,9 @@ template <class T>
 struct Pack<T, 1> {
     T raw;
     __device__ __forceinline__ void load(const T* p) { raw = __ldg(p); }
-    __device__ __forceinline__ void copy(const T* p) {
-        if constexpr (sizeof(T) == 4)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(this))), "l"(p)
-                         : "memory");
-        else
-            raw = __ldg(p);
-    }
     __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = to_float(raw); }
     __device__ __forceinline__ float most() const { return to_float(raw); }
     __device__ __forceinline__ void finite(float (&f)[1]) const { f[0] = max_nan(to_float(raw), kMasked); }
-    __device__ __forceinline__ void raise(const Pack& o) { raw = to_float(o.raw) > to_float(raw) || raw != raw ? o.raw : raw; }
     __device__ __forceinline__ void masked() { raw = from_float<T>(-CUDART_INF_F); }
 };
 
