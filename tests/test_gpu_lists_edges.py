@@ -385,3 +385,106 @@ def test_a_constant_on_a_teacher_s_logits_changes_nothing(backend, sizes):  # no
     if not uneven:
         near = type(near)(near.loss[:9], near.gradient[:9])
         check_distill(scores[:9], TeacherTop(teacher.ids[:9], logits[:9], None, 1.7), near)
+
+
+# ---- every entry once ----------------------------------------------------------------------------------------------
+
+
+def borders(n, per, rng, count):
+    """Entries at which a list is cut between CTAs, threads and batches of their loads (`per` entries a 16-byte vector, the
+    first of them at any of the list's first entries), and those beside them; `count` of them."""
+    at = {0, 1, n - 1, n - 2, n // 2}
+    for head in range(per):
+        vectors = max(0, (n - head) // per)
+        at.add(head)
+        at.add(head + vectors * per)
+        for shares in (2, 4, 8):
+            at.update(head + vectors * k // shares * per for k in range(1, shares))
+        for threads in (128, 256, 512):
+            at.update(range(head, n, threads * per))
+            at.update(range(head, n, threads * per * 4))
+    at = sorted({k for a in at for k in (a - 1, a, a + 1) if 0 <= k < n})
+    return rng.choice(at, min(count, len(at)), replace=False)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("type_,lists,width,pad", [
+    ("f32", 8, 600, 1), ("bf16", 8, 1001, 0), ("f32", 40, 3001, 3), ("bf16", 170, 5000, 1), ("f16", 160, 9003, 5),
+    ("bf16", 40, 33000, 0), ("f32", 6, 40001, 2), ("bf16", 160, 40003, 1), ("f32", 170, 19000, 1), ("bf16", 4, 150_000, 3),
+    ("f32", 2, 300_007, 1), ("bf16", 160, 140_001, 0)])
+def test_every_entry_counts_once(backend, type_, lists, width, pad, rest):  # noqa: F811
+    """All of a list's mass on 24 entries at the cuts between CTAs, threads and batches: one that is left out, or counted
+    twice, changes the sums by a twenty-fourth. Runs of the same lengths too."""
+    rng = np.random.RandomState(width + rest)
+    per = 4 if type_ == "f32" else 8
+    z = np.full((lists, width), -60.0)
+    top = np.zeros((lists, 6), np.int32)
+    for i in range(lists):
+        at = borders(width, per, rng, 24)
+        z[i, at] = rng.randint(-4, 5, len(at)) / 4
+        top[i] = rng.choice(at, 6, replace=False)  # named by the teacher; with the rest, left out of the sum outside
+    flat = torch.zeros(lists * (width + pad) + 1, dtype=TYPES[type_], device="cuda")
+    scores = flat[1:].view(lists, width + pad)[:, :width]
+    scores.copy_(torch.from_numpy(z))
+    given = torch.from_numpy(top).cuda()
+    logits = torch.from_numpy(rng.randn(lists, 6)).float().cuda()
+    log_sum = torch.logsumexp(logits.double(), 1).float() + 0.5 if rest else None
+    teacher = TeacherTop(given, logits, log_sum)
+    boundaries = torch.from_numpy((np.arange(lists + 1) * width).astype(np.int32)).cuda()
+    for s, b in ((scores, None), (scores.contiguous().flatten(), boundaries)):
+        few = slice(0, 6)
+        lp = backend.log_probs(s, given=given, top=8, boundaries=b)
+        check_log_probs(scores[few], rows_of(scores[few]), top[few], 8, 1.0,
+                        type(lp)(*[v[few] for v in (lp.given, lp.entropy, lp.log_sum, lp.top_ids, lp.top)]))
+        some = TeacherTop(given[few], logits[few], None if log_sum is None else log_sum[few])
+        for gradient in (False, True):
+            got = backend.distill(s, teacher, boundaries=b, gradient=gradient, hessian=gradient)
+            parts = [None if v is None else v.view(lists, -1)[few] for v in (got.gradient, got.hessian)]
+            check_distill(scores[few], some, type(got)(got.loss[few], *parts), None, None, type_)
+
+
+# ---- runs of 16-bit scores, and the longest lists ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("type_", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", [[0, 1, 0, 3, 0], [5] * 40, [1, 32, 33, 512, 513, 1024, 1025, 0, 7, 2000, 65, 4097, 1],
+                                   [20000, 3, 9000, 1, 1], [700] * 200, [6001] * 160])
+def test_runs_of_16_bit_scores(backend, sizes, type_, rest):  # noqa: F811
+    rng = np.random.RandomState(len(sizes) + rest)
+    bounds = np.concatenate([[0], np.cumsum(sizes)])
+    scores = torch.from_numpy(rng.randn(bounds[-1]) * 3).to(TYPES[type_]).cuda()
+    boundaries = torch.from_numpy(bounds.astype(np.int32)).cuda()
+    teacher = random_teacher(rng, sizes, 40, type_, rest, 0.9)
+    few = 14
+    ids = np.stack([[max(n - 1, 0), n] for n in sizes]).astype(np.int32)
+    lp = backend.log_probs(scores, given=torch.from_numpy(ids).cuda(), top=40, temperature=0.9, boundaries=boundaries)
+    check_log_probs(scores, rows_of(scores, bounds[: few + 1]), ids, 40, 0.9, lp)
+    got = backend.distill(scores, teacher, boundaries=boundaries, hessian=True)
+    some = TeacherTop(teacher.ids[:few], teacher.logits[:few], None if teacher.log_sum is None else teacher.log_sum[:few], 0.9)
+    check_distill(scores, some, got, None, bounds[: few + 1], type_)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("type_,lists,width,uneven", [
+    ("f32", 3, 500_003, False), ("bf16", 2, 1_000_001, False), ("f32", 150, 80_001, True), ("f32", 2, 700_000, True),
+    ("f32", 150, 80_001, False)])
+def test_the_longest_lists(backend, type_, lists, width, uneven, rest):  # noqa: F811
+    """Lists that shared memory does not hold, shares of more than 65,536 entries, and a teacher whose indices lie 65,536
+    and its multiples apart; the rest beside them counts."""
+    rng = np.random.RandomState(width + rest)
+    scores = torch.from_numpy((rng.randn(lists, width) * 2).astype(np.float32)).to(TYPES[type_]).cuda()
+    base = np.array([5, 65_536 + 5, 17, 65_536 + 6, 2 * 65_536 + 5, 65_536 + 17, 70_000, 4_464])
+    ids = np.stack([np.where(base + i < width, base + i, i) for i in range(lists)]).astype(np.int32)
+    ids[1, 3] = ids[1, 0]
+    logits = torch.from_numpy(rng.randn(lists, 8)).float().cuda()
+    log_sum = torch.logsumexp(logits.double(), 1).float() + 0.6 if rest else None
+    teacher = TeacherTop(torch.from_numpy(ids).cuda(), logits, log_sum)
+    boundaries = torch.from_numpy((np.arange(lists + 1) * width).astype(np.int32)).cuda() if uneven else None
+    s = scores.flatten() if uneven else scores
+    few = slice(0, 2)
+    some = TeacherTop(teacher.ids[few], logits[few], None if log_sum is None else log_sum[few])
+    for gradient in (False, True):
+        got = backend.distill(s, teacher, boundaries=boundaries, gradient=gradient, hessian=gradient)
+        parts = [None if v is None else v.view(lists, -1)[few] for v in (got.gradient, got.hessian)]
+        check_distill(scores[few], some, type(got)(got.loss[few], *parts), None, None, type_)
