@@ -8,7 +8,7 @@
 //            w / T p_j (Q - r / P)          elsewhere
 //   hess_j = w / T^2 Q p_j (1 - p_j)        (the diagonal of the softmax's own second derivative)
 // P is summed over the entries outside the top, not taken as 1 - sum p: a student that has learned its teacher keeps
-// little there. Where that is less than 2^-40, the entries outside go about their own maximum in a pass of their own: f32
+// little there. Where that is less than 2^-64, the entries outside go about their own maximum in a pass of their own: f32
 // holds the gradient's r p_j / P however small P is. The top's entries are marked in a bitmap, which the sum skips; their
 // gradients are written once the others are, over what the common formula left there. An entry named twice has its q added
 // in the teacher's order.
@@ -46,9 +46,10 @@ constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
 constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
 
-// Share of the student's mass outside the top below which that part is taken about its own maximum: terms below 2^-126
-// are 0, and those above are still 2^-86 of it.
-constexpr float kApart = 0x1p-40f;
+// Share of the student's mass outside the top below which that part is taken about its own maximum. Terms below 2^-126 are
+// 0: of up to 2^31 entries, a part of 2^-64 that rounding could not see. The further pass makes 4096 x 32000 bf16 lists of
+// that kind 266 us instead of 115.
+constexpr float kApart = 0x1p-64f;
 // ... and P's binary exponent from which it counts as none, as in 64 bits.
 constexpr float kNoMass = -1074.0f;
 
@@ -299,10 +300,10 @@ __device__ __forceinline__ void share_of(const Walk<T, kVec>& w, uint32_t share,
 }
 
 // What is left of a list once its sums are known and little mass lies outside the top (Shared::apart): the loss and all
-// derivatives, the entries outside the top about their own maximum.
+// derivatives, the entries outside the top about their own maximum. `data`: the thread's held vectors, or null.
 template <class T, int kVec, int kThreads, bool kCluster>
-__device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const uint32_t* bits, const DistillArgs& a, uint32_t i, uint32_t share,
-                                          uint32_t shares, Maxima most) {
+__device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const Pack<T, kVec>* data, const uint32_t* bits, const DistillArgs& a,
+                                          uint32_t i, uint32_t share, uint32_t shares, Maxima most) {
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
     uint64_t first;
     uint32_t n;
@@ -312,17 +313,27 @@ __device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const uint32_t* b
     share_of<T, kVec, kCluster>(w, share, shares, from, to);
     const float c = __fmul_rn(kLog2E, a.inv_t), weight = a.weight != nullptr ? a.weight[i] : 1.0f, m = s.joined_m, sum = s.sum;
     const uint32_t edge_at = share == 0 && t < 2 * kVec ? w.edge(t) : n;
+    auto get = [&](uint32_t v, float(&x)[kVec]) {
+        Pack<T, kVec> p;
+        if (data != nullptr)
+            p = data[v - from];
+        else
+            p.load(w.z + w.at(v));
+        p.values(x);
+    };
+    auto at_edge = [&](auto f) {
+        if (edge_at < n && ((s.edge_bits >> t) & 1u) == 0) f(to_float(w.z[edge_at]), edge_at);
+    };
     auto each = [&](auto f) {
         for (uint32_t v = from + t; v < to; v += kThreads) {
             const uint32_t skip = marks_of(s, bits, bits != nullptr, w, from, to, a.t.top, v);
-            Pack<T, kVec> p;
             float x[kVec];
-            p.load(w.z + w.at(v));
-            p.values(x);
+            get(v, x);
+#pragma unroll
             for (int e = 0; e < kVec; ++e)
                 if (((skip >> e) & 1u) == 0) f(x[e], w.at(v) + e);
         }
-        if (edge_at < n && ((s.edge_bits >> t) & 1u) == 0) f(to_float(w.z[edge_at]), edge_at);
+        at_edge(f);
     };
     float rest_m = -CUDART_INF_F, rest_sum = 0.0f;
     each([&](float z, uint32_t) { rest_m = fmaxf(rest_m, z); });
@@ -359,7 +370,31 @@ __device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const uint32_t* b
         const float p = pow2(exponent(z, m, c)) * inv_s;
         put<T>(a, out + j, first + j, (mass * p - less) * scale, hessian_of(mass * scale * a.inv_t, p), true, most);
     };
-    each([&](float z, uint32_t j) { put_one(z, j, some ? pull * pow2(exponent(z, rest_m, c)) : 0.0f); });
+    auto less_of = [&](float z) { return some ? pull * pow2(exponent(z, rest_m, c)) : 0.0f; };
+    auto put_rest = [&](float z, uint32_t j) { put_one(z, j, less_of(z)); };
+    bool whole = kVec > 1;  // whole vectors, over which the top's own go
+    if constexpr (kVec > 1) {
+        T* const grad = a.grad != nullptr ? static_cast<T*>(a.grad) + out + w.at(from) : nullptr;
+        T* const hess = a.hess != nullptr ? static_cast<T*>(a.hess) + out + w.at(from) : nullptr;
+        whole = ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(hess)) & 15) == 0;
+        if (whole) {
+            for (uint32_t v = t; v < to - from; v += kThreads) {
+                float x[kVec], h[kVec];
+                get(from + v, x);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const float p = pow2(exponent(x[e], m, c)) * inv_s;
+                    h[e] = hessian_of(mass * scale * a.inv_t, p);
+                    x[e] = (mass * p - less_of(x[e])) * scale;
+                }
+                if (grad != nullptr) __stcs(reinterpret_cast<uint4*>(grad) + v, packed<T, kVec>(x));
+                if (hess != nullptr) __stcs(reinterpret_cast<uint4*>(hess) + v, packed<T, kVec>(h));
+            }
+            at_edge(put_rest);
+        }
+    }
+    if (!whole) each(put_rest);
+    __syncthreads();
     if (t < a.t.top && s.id[t] >= 0) {  // the top's own in this share, the first that names an index with all their q
         const uint32_t id = static_cast<uint32_t>(s.id[t]);
         bool leads = id < w.head || id >= w.tail() ? share == 0 : (id - w.head) / kVec >= from && (id - w.head) / kVec < to;
@@ -600,7 +635,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
     }
     __syncthreads();
     if (s.apart != 0) {  // (every share of a cluster joins the same sums)
-        most = rest_apart<T, kVec, kThreads, kCluster>(s, bits, a, i, share, shares, most);
+        most = rest_apart<T, kVec, kThreads, kCluster>(s, kVec > 1 && held_here ? data : nullptr, bits, a, i, share, shares, most);
         if constexpr (kCluster) cg::this_cluster().sync();  // the shares' memory is read
         return;
     }
