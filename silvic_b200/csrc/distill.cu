@@ -47,8 +47,8 @@ constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three 
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
 
 // Share of the student's mass outside the top below which that part is taken about its own maximum. Terms below 2^-126 are
-// 0: of up to 2^31 entries, a part of 2^-64 that rounding could not see. The further pass makes 4096 x 32000 bf16 lists of
-// that kind 266 us instead of 115.
+// 0: of up to 2^31 entries at most 2^-31 of that share, less than a rounding. The further pass makes 4096 x 32000 bf16 lists
+// of that kind 266 us instead of 115.
 constexpr float kApart = 0x1p-64f;
 // ... and P's binary exponent from which it counts as none, as in 64 bits.
 constexpr float kNoMass = -1074.0f;

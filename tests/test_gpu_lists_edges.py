@@ -488,3 +488,47 @@ def test_the_longest_lists(backend, type_, lists, width, uneven, rest):  # noqa:
         got = backend.distill(s, teacher, boundaries=boundaries, gradient=gradient, hessian=gradient)
         parts = [None if v is None else v.view(lists, -1)[few] for v in (got.gradient, got.hessian)]
         check_distill(scores[few], some, type(got)(got.loss[few], *parts), None, None, type_)
+
+
+# ---- graphs over every way of working ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("type_,lists,width,uneven", [
+    ("f32", 40, 300, False), ("bf16", 40, 900, False), ("f32", 300, 20_011, False), ("bf16", 3, 150_001, False),
+    ("bf16", 160, 33_000, False), ("f32", 2, 500_003, False), ("f32", 40, 200, True), ("f32", 30, 5_000, True),
+    ("bf16", 2, 60_000, True)])
+def test_graphs_replay_every_way_of_working(backend, type_, lists, width, uneven):  # noqa: F811
+    """A graph captured on ordinary scores is replayed on a confident student's, on masked lists and on far scores, beside
+    eager calls on the same inputs."""
+    rng = np.random.RandomState(width)
+    x = torch.randn(lists, width, device="cuda").to(TYPES[type_])
+    teacher = random_teacher(rng, [width] * lists, 20, "f32", True)
+    given = teacher.ids[:, :3].contiguous()
+    boundaries = (torch.arange(lists + 1, device="cuda") * width).int() if uneven else None
+    s = x.flatten() if uneven else x
+    assert s.data_ptr() == x.data_ptr()
+
+    def calls():
+        lp = backend.log_probs(s, given=given, top=30, boundaries=boundaries)
+        return [lp.given, lp.entropy, lp.log_sum, lp.top_ids, lp.top,
+                *[v for gradient in (False, True)
+                  for d in [backend.distill(s, teacher, boundaries=boundaries, gradient=gradient, hessian=gradient)]
+                  for v in (d.loss, d.gradient, d.hessian) if v is not None]]
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    for turn in range(4):
+        x.copy_(torch.randn(lists, width, device="cuda"))
+        if turn == 1:
+            x.scatter_(1, teacher.ids.long(), 200.0)
+        if turn == 2:
+            x[:, : width // 2] = -np.inf
+            x[0] = -np.inf
+        if turn == 3:
+            x.mul_(3.0e6)
+        graph.replay()
+        for got, want in zip(out, calls()):
+            assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
