@@ -19,15 +19,15 @@
 // where it starts. A dense list too long for shared memory, or of scores so far from 0 that fma(z, c, -m c) loses its last bits,
 // is read again for each pass. The loss alone is taken in one pass that holds nothing.
 //
-// What bounds it, on one B200 (copy rate 6453 GB/s): 4096 lists of 32000 bf16 scores, top 64 with the rest, take 120 us,
-// 4.4 TB/s, 0.68 of the copy rate; 2048 lists of 131072 (clusters of 4), top 100, 260 us, 0.64. Each score's exponential is
+// What bounds it, on one B200 (copy rate 6453 GB/s): 4096 lists of 32000 bf16 scores, top 64 with the rest, take 123 us,
+// 4.3 TB/s, 0.66 of the copy rate; 2048 lists of 131072 (clusters of 4), top 100, 255 us, 0.65. Each score's exponential is
 // taken twice, 128 cycles of the special-function unit for a warp's vector of 8, beside about 85 instructions; that unit is
-// 48% busy, issue 50%, and the list's five barriers take a quarter of the warps' waiting. Holding the list in registers
+// 47% busy, issue 50%, and the list's five barriers take a quarter of the warps' waiting. Holding the list in registers
 // instead of shared memory left one CTA of 512 threads or spilled (wide: 387 us); reading it twice from L2 took 265 us on
 // the wide lists and 153 on the others, where shared memory took 277 and 131 at the time. CTAs of half a list (36 KB)
 // repeat the scalars (150 us and 269), CTAs of 512 threads lose to their barriers (208 and 321). The next list's copies,
 // begun as each slot's gradient is written, gain 2%: memory's latency is not what is left.
-// The loss alone over 1500 lists of 50257 f16 takes 42 us, 3.6 TB/s; 16,700 lists of 120 f32 with gradient and hessian, a
+// The loss alone over 1500 lists of 50257 f16 takes 43 us, 3.5 TB/s; 16,700 lists of 120 f32 with gradient and hessian, a
 // warp each, 17 us, bound by the chain of loads and reductions of a list.
 #include <algorithm>
 
@@ -43,7 +43,11 @@ namespace {
 // of 300 take 24 us so and 71 by a CTA each; of widely spread lengths about 300, 70 and 75, about 440, 54 and 42.
 constexpr uint32_t kWarpMean = 384;
 constexpr int kWarpThreads = 256;    // the warp kernel's CTAs
-constexpr uint32_t kHeld = 73728;    // bytes of scores that a CTA holds: three CTAs' worth fits an SM
+// Bytes of scores that a CTA holds; a longer list takes more shares. Beside them lie the marks (a sixteenth of 16-bit scores)
+// and the static memory, so three CTAs fit an SM up to 70,700 bytes of bf16 and two above: lists of 35,000 (131M scores in
+// all) take 119 us, of 36,800 134 (162 in twice the shares). Past it, 37,000 take 172 us in two shares; one share and two
+// CTAs an SM would take 141.
+constexpr uint32_t kHeld = 73728;
 constexpr int kMaxHeld = 216 * 1024; // and the most, with the marks, beside the static shared memory
 
 // Share of the student's mass outside the top below which that part is taken about its own maximum. Terms below 2^-126 are
@@ -174,12 +178,21 @@ __device__ __forceinline__ void teacher_entry(const DistillArgs& a, uint32_t i, 
     y = id >= 0 ? load_typed(a.t.logits, a.t.type, at) : -CUDART_INF_F;
 }
 
-// The loss of a list from its parts: sum q (log q - (z - m) / T), sum q, S, log (S P), and the rest.
-__device__ __forceinline__ float loss_of(float cross, float held, float sum, float log_outside, float r) {
+// The loss's cross terms are summed at 2^-32 of themselves (exactly): a teacher's entry that the student masks by the type's
+// lowest value makes one of about 2^128 / T, which the loss may still hold once it is multiplied by q.
+constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;
+
+// One of them, q (log q - (z - m) / T).
+__device__ __forceinline__ float cross_term(float q, float log_q, float z, float m, float inv_t) {
+    return q != 0.0f ? q * (log_q * kDown - (z * kDown - m * kDown) * inv_t) : 0.0f;
+}
+
+// The loss of a list from its weight and its parts: the cross terms, sum q, S, log (S P), and the rest.
+__device__ __forceinline__ float loss_of(float weight, float cross, float held, float sum, float log_outside, float r) {
     const float log_s = logf(sum);
-    float loss = cross + held * log_s;
+    float loss = held * log_s;
     if (r > 0.0f) loss += r * (logf(r) - (log_outside - log_s));
-    return loss;
+    return weight * cross * kUp + weight * loss;
 }
 
 // Whether a maximum outside the top leaves P a mass: less than 64 bits hold counts as none, as a masked entry's.
@@ -362,7 +375,7 @@ __device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const Pack<T, kVe
     }
     const float r = some ? s.r : 0.0f;
     if (t == 0 && share == 0 && a.loss != nullptr)
-        a.loss[i] = weight * loss_of(s.cross, s.held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
+        a.loss[i] = loss_of(weight, s.cross, s.held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
     if (a.grad == nullptr && a.hess == nullptr) return most;
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
     const float mass = s.held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
@@ -557,7 +570,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         s.q[t] = q;
         const float top_part = warp_sum(rest && leads ? term(zt) : 0.0f);
         const float held_part = warp_sum(q);
-        const float cross_part = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
+        const float cross_part = warp_sum(cross_term(q, log_q, zt, m, a.inv_t));
         if (lane == 0) {
             s.warp[3][warp] = top_part;
             s.warp[4][warp] = held_part;
@@ -592,7 +605,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
             const float all = warp_max(other_m), f = pow2(exponent(other_m, all, c));
             outside = warp_sum(lane < shares ? other_outside * f : 0.0f);
             top_sum = warp_sum(lane < shares ? other_top * f : 0.0f);
-            if (held != 0.0f) cross += held * ((all - m) * a.inv_t);  // (a masked share's m is so low that this may be 0 times inf)
+            cross += held * ((all * kDown - m * kDown) * a.inv_t);
             m = all;
         }
     }
@@ -601,7 +614,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
         float q_scale = 1.0f;
         if (!rest && held != 0.0f) {
             q_scale = 1.0f / held;
-            cross = cross * q_scale - logf(held);
+            cross = cross * q_scale - logf(held) * kDown;
             held = 1.0f;
         }
         const float r = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
@@ -629,7 +642,7 @@ __device__ __forceinline__ void distill_list(Shared<kThreads>& s, Pack<T, kVec>*
                 s.cross = cross;
                 s.r = r;
             } else if (share == 0 && a.loss != nullptr) {
-                a.loss[i] = none ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), r);
+                a.loss[i] = none ? 0.0f : loss_of(weight, cross, held, sum, logf(outside), r);
             }
         }
     }
@@ -863,7 +876,7 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
         const float log_q = log_q_of(y, a.inv_t, rest, log_sum, y_max), q = id >= 0 ? expf(log_q) : 0.0f;
         const float top_part = warp_sum(rest && leads ? pow2(exponent(zt, m, c)) : 0.0f);
         const float held_part = warp_sum(q);
-        const float cross_part = warp_sum(q != 0.0f ? q * (log_q - (zt - m) * a.inv_t) : 0.0f);
+        const float cross_part = warp_sum(cross_term(q, log_q, zt, m, a.inv_t));
         if (lane == 0) {
             s.warp[3][warp] = top_part;
             s.warp[4][warp] = held_part;
@@ -905,12 +918,12 @@ __device__ __forceinline__ bool loss_list(Shared<kThreads>& s, uint32_t* bits, c
     const float sum = outside + top_sum, rest_q = rest ? fmaxf(1.0f - held, 0.0f) : 0.0f;
     if (far || (rest_q > 0.0f && sum != 0.0f && taught && outside < kApart * sum)) return false;
     if (t == 0 && share == 0) {
-        if (held != 0.0f) cross += held * ((all - m) * a.inv_t);  // (a masked first batch's m is so low that this may be 0 times inf)
+        cross += held * ((all * kDown - m * kDown) * a.inv_t);
         if (!rest && held != 0.0f) {
-            cross = cross / held - logf(held);
+            cross = cross / held - logf(held) * kDown;
             held = 1.0f;
         }
-        a.loss[i] = sum == 0.0f || !taught ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), rest_q);
+        a.loss[i] = sum == 0.0f || !taught ? 0.0f : loss_of(weight, cross, held, sum, logf(outside), rest_q);
     }
     return true;
 }
@@ -976,7 +989,7 @@ __device__ __noinline__ Maxima warp_rest_apart(const WarpShared& s, const Distil
     const float r = some ? 1.0f - held : 0.0f;
     cross = warp_sum(cross);
     if (lane == 0 && a.loss != nullptr)
-        a.loss[i] = weight * loss_of(cross, held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
+        a.loss[i] = loss_of(weight, cross, held, sum, (rest_m - m) * a.inv_t + logf(rest_sum), r);
     if (a.grad == nullptr && a.hess == nullptr) return most;
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
     const float mass = held + r, scale = weight * a.inv_t, inv_s = 1.0f / sum, pull = some ? r / rest_sum : 0.0f;
@@ -1084,7 +1097,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
         if (id[u] >= 0 && (rest || total != 0.0f)) log_q = log_q_of(y[u], a.inv_t, rest, log_sum, y_max) - (rest ? 0.0f : log_total);
         q[u] = expf(log_q);
         held += q[u];
-        if (q[u] != 0.0f) cross += q[u] * (log_q - (zt[u] - m) * a.inv_t);
+        cross += cross_term(q[u], log_q, zt[u], m, a.inv_t);
         if (u * 32 + lane < a.t.top) s.q[u * 32 + lane] = q[u];
     }
     held = warp_sum(held);
@@ -1098,7 +1111,7 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
     }
     if (a.loss != nullptr) {
         cross = warp_sum(cross);
-        if (lane == 0) a.loss[i] = empty ? 0.0f : weight * loss_of(cross, held, sum, logf(outside), r);
+        if (lane == 0) a.loss[i] = empty ? 0.0f : loss_of(weight, cross, held, sum, logf(outside), r);
     }
     if (a.grad == nullptr && a.hess == nullptr) return;
     const uint64_t out = a.l.bounds != nullptr ? first : static_cast<uint64_t>(i) * a.grad_stride;
@@ -1245,7 +1258,7 @@ void launch_typed(const DistillArgs& a, cudaStream_t s) {
     }
     uint32_t shares = list_shares(mean, a.l.lists, a.sms);
     if (a.l.bounds != nullptr) {
-        if (mean / shares <= 1024)
+        if (mean / shares <= 1024)  // (8M scores, f32: lists of 1000 by 128 threads 60 us, by 256 102; of 4000, 39 and 49)
             launch_rows<T, 1, 128>(a, shares, 0, s);
         else
             launch_rows<T, 1, 256>(a, shares, 0, s);
@@ -1253,7 +1266,7 @@ void launch_typed(const DistillArgs& a, cudaStream_t s) {
     }
     if (a.grad == nullptr && a.hess == nullptr) {
         if (a.loss == nullptr) return;
-        if (mean / shares <= 4096)
+        if (mean / shares <= 4096)  // (64M scores, bf16: lists of 4000 by 128 threads 67 us, by 256 103; of 16000, 39 and 46)
             launch_loss<T, kVec, 128>(a, shares, mean, s);
         else
             launch_loss<T, kVec, 256>(a, shares, mean, s);
@@ -1264,6 +1277,8 @@ void launch_typed(const DistillArgs& a, cudaStream_t s) {
     while (shares < 8 && bytes > static_cast<uint64_t>(shares) * kHeld) shares *= 2;
     uint64_t slots = (mean / kVec + shares - 1) / shares;
     if (rows_smem<T, kVec>(static_cast<uint32_t>(std::min<uint64_t>(slots, kMaxHeld / 16))) > kMaxHeld) slots = 0;
+    // (f32, 32M scores: lists of 4000 by 128 threads 67 us, by 256 92; of 16000, 71 and 58. bf16, 64M: of 4000, 109 and 174; of
+    // 16000, 62 and 74: the border lies between 4096 entries and 64 KB.)
     if (mean / shares <= 4096)
         launch_rows<T, kVec, 128>(a, shares, static_cast<uint32_t>(slots), s);
     else

@@ -532,3 +532,48 @@ def test_graphs_replay_every_way_of_working(backend, type_, lists, width, uneven
         graph.replay()
         for got, want in zip(out, calls()):
             assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
+# ---- a teacher's entries that the student masks by the type's lowest value -------------------------------------------
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("t", [1.0, 0.3, 0.05])
+@pytest.mark.parametrize("type_,lists,width,uneven", [
+    ("f32", 9, 40, False), ("bf16", 9, 900, False), ("f32", 300, 5_001, False), ("bf16", 3, 40_001, False),
+    ("f32", 9, 300, True), ("bf16", 160, 1_501, True)])
+def test_the_loss_of_entries_masked_by_the_lowest_value(backend, type_, lists, width, uneven, t, rest):  # noqa: F811
+    """Losses of up to f32's largest, from terms beyond it; past it, infinite."""
+    rng = np.random.RandomState(width)
+    z = rng.randn(lists, width) * 3
+    z[rng.rand(lists, width) < 0.5] = torch.finfo(TYPES[type_]).min
+    z[:, :3] = 2.0
+    scores = torch.from_numpy(z).to(TYPES[type_]).cuda()
+    ids = np.stack([rng.choice(width, 5, replace=False) for _ in range(lists)]).astype(np.int32)
+    logits = rng.randn(lists, 5) * t
+    for i in range(lists):  # masked ones with 2^-1 to 2^-40 of the teacher's mass, the first with most of it
+        z[i, ids[i, 0]] = 1.0
+        masked = [k for k in range(1, 5) if z[i, ids[i, k]] < -1e30]
+        logits[i, masked] -= rng.choice([0.5, 5.0, 28.0]) * t
+    scores = torch.from_numpy(z).to(TYPES[type_]).cuda()
+    logits = torch.from_numpy(logits).float()
+    log_sum = torch.logsumexp(logits.double() / t, 1).float() + 0.4 if rest else None
+    teacher = TeacherTop(torch.from_numpy(ids).cuda(), logits.cuda(), None if log_sum is None else log_sum.cuda(), t)
+    boundaries = (torch.arange(lists + 1, device="cuda") * width).int() if uneven else None
+    finite = 0
+    for weight, gradient in ((1.0, False), (1.0, True), (0.125, False), (0.125, True)):
+        got = backend.distill(scores.flatten() if uneven else scores, teacher, boundaries=boundaries, gradient=gradient,
+                              weight=torch.full((lists,), weight, device="cuda"))
+        for i in range(9 if lists > 9 else lists):
+            want = ref.distill(rows_of(scores[i: i + 1])[0], ids[i], logits[i].numpy(), t,
+                               None if log_sum is None else float(log_sum[i]), weight)
+            loss = float(got.loss[i])
+            if want["loss"] > 3.5e38:
+                assert loss == np.inf
+            elif want["loss"] < 3.3e38:
+                # q is off by 4 U and by its argument's rounding, a term by three roundings more, a sum of five by three
+                arg = np.abs(logits[i].numpy()).max() / t + (0.0 if log_sum is None else abs(float(log_sum[i])))
+                tol = 2 * (16 + 4 * arg) * ref.U * want["terms"] + 4 * ref.slack(width) * want["terms"]
+                assert abs(loss - want["loss"]) <= tol, (loss, want["loss"])
+                finite += want["loss"] > 1e20
+    assert finite > 0 or lists < 9
