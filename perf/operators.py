@@ -279,6 +279,9 @@ def run(state):
     if c["op"] == "log_probs":
         r = _backend().log_probs(state["scores"], given=state["ids"], top=c["top"], temperature=state["temperature"],
                                  boundaries=state["boundaries"])
+        if not c["top"]:  # no alternatives: the call gives None, the plain form tensors without columns
+            none = state["ids"].new_empty((c["lists"], 0))
+            return dict(given=r.given, entropy=r.entropy, log_sum=r.log_sum, top_ids=none, top=none.float())
         return dict(given=r.given, entropy=r.entropy, log_sum=r.log_sum, top_ids=r.top_ids, top=r.top)
     from silvic_b200 import TeacherTop
 
