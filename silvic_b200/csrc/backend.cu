@@ -2317,7 +2317,8 @@ int list_args(sb2_backend* b, const sb2_lists* lists, ListsArgs& a) {
             return b->fail(SB2_EUNSUPPORTED, std::to_string(lists->width) + " entries behind boundaries; the limit is 2^31 - 1");
         SB2_TRY(check_memory(b, lists->boundaries_dev, "the boundaries"));
     }
-    if (lists->num_lists > 0 && lists->width > 0) SB2_TRY(check_memory(b, lists->scores_dev, "the scores", type_bytes(lists->type)));
+    if (lists->num_lists > 0 && lists->width > 0)
+        SB2_TRY(check_memory(b, lists->scores_dev, "the scores", type_bytes(lists->type)));
     a.scores = lists->scores_dev;
     a.type = lists->type;
     a.lists = lists->num_lists;

@@ -315,8 +315,8 @@ __device__ __forceinline__ void share_of(const Walk<T, kVec>& w, uint32_t share,
 // What is left of a list once its sums are known and little mass lies outside the top (Shared::apart): the loss and all
 // derivatives, the entries outside the top about their own maximum. `data`: the thread's held vectors, or null.
 template <class T, int kVec, int kThreads, bool kCluster>
-__device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const Pack<T, kVec>* data, const uint32_t* bits, const DistillArgs& a,
-                                          uint32_t i, uint32_t share, uint32_t shares, Maxima most) {
+__device__ __noinline__ Maxima rest_apart(Shared<kThreads>& s, const Pack<T, kVec>* data, const uint32_t* bits,
+                                          const DistillArgs& a, uint32_t i, uint32_t share, uint32_t shares, Maxima most) {
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
     uint64_t first;
     uint32_t n;
@@ -971,8 +971,8 @@ struct WarpShared {
 
 // rest_apart() of a warp's list (`cross`: a lane's part).
 template <class T>
-__device__ __noinline__ Maxima warp_rest_apart(const WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n, float m,
-                                               float sum, float held, float cross, Maxima most) {
+__device__ __noinline__ Maxima warp_rest_apart(const WarpShared& s, const DistillArgs& a, uint32_t i, uint64_t first, uint32_t n,
+                                               float m, float sum, float held, float cross, Maxima most) {
     const uint32_t lane = threadIdx.x & 31;
     const T* z = static_cast<const T*>(a.l.scores) + first;
     const float c = __fmul_rn(kLog2E, a.inv_t), weight = a.weight != nullptr ? a.weight[i] : 1.0f;
@@ -1094,7 +1094,8 @@ __device__ __forceinline__ void distill_warp(WarpShared& s, const DistillArgs& a
 #pragma unroll
     for (int u = 0; u < kTop; ++u) {
         float log_q = -CUDART_INF_F;
-        if (id[u] >= 0 && (rest || total != 0.0f)) log_q = log_q_of(y[u], a.inv_t, rest, log_sum, y_max) - (rest ? 0.0f : log_total);
+        if (id[u] >= 0 && (rest || total != 0.0f))
+            log_q = log_q_of(y[u], a.inv_t, rest, log_sum, y_max) - (rest ? 0.0f : log_total);
         q[u] = expf(log_q);
         held += q[u];
         cross += cross_term(q[u], log_q, zt[u], m, a.inv_t);

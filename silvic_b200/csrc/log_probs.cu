@@ -12,12 +12,12 @@
 // ascending order, or of equal scores) have the alternatives selected digit by digit of their keys.
 //
 // What bounds it, on one B200 (copy rate 6453 GB/s): 4096 lists of 131072 bf16 scores, top 20, take 257 us, 4.2 TB/s,
-// 0.65 of the copy rate (243 us where one input is repeated, as in the comparisons below). Per vector of 8 scores a warp issues about 65 instructions and its exponentials take the
-// special-function unit 64 cycles; issue is 64% busy, that unit 51%, DRAM 48% under the profiler (1184 lists). Read
-// the list twice (maximum first) and L2 would carry it once more; so one pass, about a reference that moves. Candidates
-// as whole vectors: testing and storing each entry cost about 100 instructions a hit, a vector costs 25. A short list's
-// time is its chain of loads, barriers and selections: one list of 131072, as a cluster of 8, takes 10 us, 16,700
-// lists of 120 f32, a warp each, 17.5 us.
+// 0.65 of the copy rate (243 us where one input is repeated, as in the comparisons below). Per vector of 8 scores a warp
+// issues about 65 instructions and its exponentials take the special-function unit 64 cycles; issue is 65% busy, that unit
+// 51%, DRAM 48% under the profiler (1184 lists). Read the list twice (maximum first) and L2 would carry it once more; so one
+// pass, about a reference that moves. Candidates as whole vectors: testing and storing each entry cost about 100
+// instructions a hit, a vector costs 25. A short list's time is its chain of loads, barriers and selections: one list of
+// 131072, as a cluster of 8, takes 10 us, 16,700 lists of 120 f32, a warp each, 17.5 us.
 #include "lists_device.cuh"
 
 namespace cg = cooperative_groups;
