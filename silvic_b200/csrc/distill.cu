@@ -192,7 +192,8 @@ __device__ __forceinline__ float loss_of(float weight, float cross, float held, 
     const float log_s = logf(sum);
     float loss = held * log_s;
     if (r > 0.0f) loss += r * (logf(r) - (log_outside - log_s));
-    return weight * cross * kUp + weight * loss;
+    const float up = cross * kUp;
+    return fabsf(up) <= FLT_MAX ? weight * (up + loss) : weight * cross * kUp + weight * loss;
 }
 
 // Whether a maximum outside the top leaves P a mass: less than 64 bits hold counts as none, as a masked entry's.

@@ -577,3 +577,18 @@ def test_the_loss_of_entries_masked_by_the_lowest_value(backend, type_, lists, w
                 assert abs(loss - want["loss"]) <= tol, (loss, want["loss"])
                 finite += want["loss"] > 1e20
     assert finite > 0 or lists < 9
+
+
+@pytest.mark.parametrize("weight", [2.0 ** -110, 2.0 ** -60, 2.0 ** 60, 2.0 ** 110])
+@pytest.mark.parametrize("lists,width,uneven", [(9, 300, False), (5, 5_000, False), (300, 5_001, False), (9, 300, True)])
+def test_a_weight_scales_the_loss_exactly(backend, lists, width, uneven, weight):  # noqa: F811
+    """A power of two, however small or large."""
+    rng = np.random.RandomState(width)
+    scores = torch.from_numpy(rng.randn(lists, width) * 2).float().cuda()
+    teacher = random_teacher(rng, [width] * lists, 7, "f32", True)
+    boundaries = (torch.arange(lists + 1, device="cuda") * width).int() if uneven else None
+    s = scores.flatten() if uneven else scores
+    for gradient in (False, True):
+        one, many = [backend.distill(s, teacher, boundaries=boundaries, gradient=gradient,
+                                     weight=torch.full((lists,), w, device="cuda")) for w in (1.0, weight)]
+        assert (one.loss.abs() > 1e-3).all() and torch.equal(many.loss, one.loss * weight)
