@@ -274,13 +274,13 @@ def test_misaligned_pointers_are_refused(backend):  # noqa: F811
     lib, h = backend._lib, backend._h
 
     def log_probs(a=lists, **at):
-        p = dict(given=ok + 1024, given_out=ok + 2048, entropy=ok + 3072, log_sum=ok + 4096, ids=ok + 5120, out=ok + 6144)
+        p = dict(given=ok + 1000, given_out=ok + 2000, entropy=ok + 3000, log_sum=ok + 4000, ids=ok + 5000, out=ok + 6000)
         p.update(at)
         return lib.sb2_log_probs(h, C.byref(a), 1.0, p["given"], 1, 2, p["given_out"], p["entropy"], p["log_sum"], p["ids"], p["out"],
                                  None)
 
     def distill(a=lists, **at):
-        p = dict(ids=ok + 1024, log_sum=ok + 2048, weight=ok + 3072, loss=ok + 4096)
+        p = dict(ids=ok + 1000, log_sum=ok + 2000, weight=ok + 3000, loss=ok + 4000)
         p.update(at)
         t = _abi.Teacher(p["ids"], ok + 512, _abi.F32, 2, 2, p["log_sum"])
         return lib.sb2_distill(h, C.byref(a), C.byref(t), 1.0, p["weight"], p["loss"], None, None, 0, None)
